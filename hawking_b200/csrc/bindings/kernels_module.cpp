@@ -362,4 +362,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   hk::register_model_kernels(m);
   hk::register_mg_kernels(m);
   hk::register_ds_kernels(m);
+  hk::register_kv4_kernels(m);
 }

@@ -8,4 +8,5 @@ void register_tp_kernels(pybind11::module_& m);
 void register_model_kernels(pybind11::module_& m);
 void register_mg_kernels(pybind11::module_& m);
 void register_ds_kernels(pybind11::module_& m);
+void register_kv4_kernels(pybind11::module_& m);
 }  // namespace hk

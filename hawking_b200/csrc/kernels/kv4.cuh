@@ -1,0 +1,50 @@
+// Inside of a unit of the 4-bit paged KV cache: 16 tokens of one kv head, 18 * HD bytes.
+//
+// A value is c + s * (code - 8): a 4-bit code, and per token and 64 head dims one float16 pair
+// (s, c): 4.5 bits a value. The codes lie in the order in which the attention kernels' matrix
+// fragments take them, so that a warp reads its operands as whole 16-byte pieces without bank
+// conflicts and a few bit operations on each 32-bit word give pairs of operands:
+//
+//   keys     words [HD / 128][token 16][t 4][i]: nibble p + 4 e = head dim 128 plane + 32 i + 8 t + 2 p + e
+//   values   words [HD / 64][g 8][t 4][i 2][h 2]: nibble p + 4 e = token 8 h + 2 t + e, dim 64 plane + 32 i + 4 g + p
+//   pairs    keys [token 16][HD / 64] (s, c), then values likewise
+//
+// (g = lane / 4 and t = lane % 4 of the mma.m16n8k16 fragments; (w & 0x000f000f) and its shifts by
+// 4, 8 and 12 are the nibble pairs (p, p + 4).)
+#pragma once
+#include "common.cuh"
+#include "kv4.h"
+
+namespace hk {
+namespace kv4 {
+
+template <int HD>
+struct Unit {
+  static constexpr int kGroups = HD / 64;                // (s, c) pairs of one token's K (or V)
+  static constexpr int kRow = (HD < 128 ? HD : 128) / 2;  // bytes of one token's key codes in a plane
+  static constexpr int kCodes = 8 * HD;                  // bytes of the key (or value) codes
+  static constexpr int kPairsK = 16 * HD;                // byte offset of the key pairs
+  static constexpr int kPairsV = 17 * HD;                // byte offset of the value pairs
+  static constexpr int kBytes = 18 * HD;
+
+  // byte of the key word holding dims [d, d + 8) (d % 8 == 0) of token `tok`
+  __host__ __device__ static constexpr int key_word(int tok, int d) {
+    return (d >> 7) * 16 * kRow + tok * kRow + ((d >> 3) & 3) * (kRow / 4) + ((d & 127) >> 5) * 4;
+  }
+  // byte of the value half word holding dims [d, d + 4) (d % 4 == 0) of token `tok`
+  __host__ __device__ static constexpr int value_half(int tok, int d) {
+    return kCodes + (d >> 6) * 512 + ((d >> 2) & 7) * 64 + ((tok & 7) >> 1) * 16 + ((d >> 5) & 1) * 8 + (tok >> 3) * 4 +
+           (tok & 1) * 2;
+  }
+  // byte of the (s, c) pair of group `grp` of token `tok`
+  __host__ __device__ static constexpr int pair(bool value, int tok, int grp) {
+    return (value ? kPairsV : kPairsK) + tok * (4 * kGroups) + grp * 4;
+  }
+};
+
+// Largest magnitude a group holds: larger finite values are clamped to it, so that the centre and
+// the ends c - 8 s, c + 7 s of every group stay finite in float16.
+constexpr float kMaxValue = 65024.f;
+
+}  // namespace kv4
+}  // namespace hk

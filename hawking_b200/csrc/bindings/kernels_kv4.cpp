@@ -179,7 +179,8 @@ void kv4_gather(const Tensor& cache, const Tensor& slots, const optional<Tensor>
 
 void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Tensor& block_tables,
                    const Tensor& row_seq, const Tensor& row_ctx, double scale, const optional<Tensor>& out,
-                   const optional<Tensor>& out_bf16, const optional<Tensor>& sinks, const Tensor& status, bool pdl) {
+                   const optional<Tensor>& out_bf16, const optional<Tensor>& sinks, const Tensor& status, const Tensor& part, const Tensor& counters,
+                   int64_t sms, bool pdl) {
   const Shape sh = cache_shape(cache);
   const at::Device dev = cache.device();
   TORCH_CHECK(q.device() == dev && q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == sh.hd &&
@@ -223,10 +224,14 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
     a.sinks = sinks->data_ptr<float>();
   }
   a.status = ints_out(status, 1, dev, "status");
+  TORCH_CHECK(part.device() == dev && part.scalar_type() == at::kFloat && part.is_contiguous() &&
+                  part.numel() >= hk::kKv4PartFloats((int)sms) && sms > 0 && 12 * sms <= hk::kKv4Counters,
+              "kv4 attention: the workspace's partials are too small");
+  const hk::Kv4Workspace ws{part.data_ptr<float>(), ints_out(counters, hk::kKv4Counters, dev, "counters"), (int)sms};
   const c10::cuda::CUDAGuard g(dev);
   const cudaStream_t s = at::cuda::getCurrentCUDAStream().stream();
   if (prefill) hk::kv4_attention_prefill_launch(a, s, pdl);
-  else hk::kv4_attention_decode_launch(a, s, pdl);
+  else hk::kv4_attention_decode_launch(a, ws, s, pdl);
 }
 
 }  // namespace
@@ -246,6 +251,8 @@ void register_kv4_kernels(py::module_& m) {
         py::arg("pdl") = false);
   m.def("kv4_attention", &kv4_attention, py::arg("prefill"), py::arg("q"), py::arg("cache"), py::arg("block_tables"),
         py::arg("row_seq"), py::arg("row_ctx"), py::arg("scale"), py::arg("out"), py::arg("out_bf16"),
-        py::arg("sinks"), py::arg("status"), py::arg("pdl") = false);
+        py::arg("sinks"), py::arg("status"), py::arg("part"), py::arg("counters"), py::arg("sms"),
+        py::arg("pdl") = false);
+  m.def("kv4_workspace_sizes", [](int64_t sms) { return std::make_pair(hk::kKv4PartFloats((int)sms), hk::kKv4Counters); });
 }
 }  // namespace hk

@@ -67,10 +67,20 @@ struct Kv4AttnArgs {
   int* status;
 };
 
+// Scratch of the attention launches of one stream. counters are zero between launches.
+struct Kv4Workspace {
+  float* part;    // kKv4PartFloats
+  int* counters;  // kKv4Counters
+  int sms;
+};
+constexpr int kKv4Counters = 2048;  // decode: three per CTA
+// decode: at most 4 CTAs per SM, two partials each of at most 16 heads x (128 + 4) or 8 x (256 + 4)
+constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * 4 * 2 * 2112; }
+
 void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl);
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl);
 void kv4_gather_launch(const Kv4GatherArgs& a, cudaStream_t s, bool pdl);
-void kv4_attention_decode_launch(const Kv4AttnArgs& a, cudaStream_t s, bool pdl);
+void kv4_attention_decode_launch(const Kv4AttnArgs& a, const Kv4Workspace& ws, cudaStream_t s, bool pdl);
 void kv4_attention_prefill_launch(const Kv4AttnArgs& a, cudaStream_t s, bool pdl);
 
 }  // namespace hk

@@ -91,7 +91,6 @@ void launch_any(const Kv4AttnArgs& a, cudaStream_t s, bool pdl) {
 
 }  // namespace
 
-void kv4_attention_decode_launch(const Kv4AttnArgs& a, cudaStream_t s, bool pdl) { launch_any(a, s, pdl); }
 void kv4_attention_prefill_launch(const Kv4AttnArgs& a, cudaStream_t s, bool pdl) { launch_any(a, s, pdl); }
 
 }  // namespace hk

@@ -45,11 +45,22 @@ def cache_shape(num_blocks: int, n_kv_heads: int, block_size: int, head_dim: int
 
 
 class Workspace:
-    """What the attention launches of one stream keep between calls: the device status word. Use one
-    workspace per stream; launches that share one must be ordered."""
+    """What the attention launches of one stream share: the device status word, the partial results of
+    rows that several CTAs work on, and their arrival counters (zero between launches). Use one
+    workspace per stream: launches that share one must be ordered."""
 
     def __init__(self, device="cuda"):
+        self.device = torch.device(device)
+        self.sms = torch.cuda.get_device_properties(self.device).multi_processor_count
+        floats, counters = kernels().kv4_workspace_sizes(self.sms)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.part = torch.empty(floats, dtype=torch.float32, device=device)
+        self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
+
+    def reset(self):
+        """Clear the status word and the counters (after a launch reported a failed wait)."""
+        self.status.zero_()
+        self.counters.zero_()
 
 
 def plan_rows(seq_rows: torch.Tensor, cached: torch.Tensor, new: torch.Tensor, block_tables: torch.Tensor,
@@ -108,7 +119,7 @@ def attention_decode(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.T
     ``[rows, heads * head_dim]``. A row with no context gives zeros."""
     launches.add()
     kernels().kv4_attention(False, q, cache, block_tables, row_seq, row_ctx, scale, out, out_bf16, sinks, ws.status,
-                            PDL)
+                            ws.part, ws.counters, ws.sms, PDL)
 
 
 def attention_prefill(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, row_seq: torch.Tensor,
@@ -118,4 +129,4 @@ def attention_prefill(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.
     ``row_ctx``; head_dim 64 or 128."""
     launches.add()
     kernels().kv4_attention(True, q, cache, block_tables, row_seq, row_ctx, scale, out, out_bf16, sinks, ws.status,
-                            PDL)
+                            ws.part, ws.counters, ws.sms, PDL)

@@ -225,7 +225,7 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
   }
   a.status = ints_out(status, 1, dev, "status");
   TORCH_CHECK(part.device() == dev && part.scalar_type() == at::kFloat && part.is_contiguous() &&
-                  part.numel() >= hk::kKv4PartFloats((int)sms) && sms > 0 && 12 * sms <= hk::kKv4Counters,
+                  part.numel() >= hk::kKv4PartFloats((int)sms) && sms > 0 && 3 * sms <= hk::kKv4Counters,
               "kv4 attention: the workspace's partials are too small");
   const hk::Kv4Workspace ws{part.data_ptr<float>(), ints_out(counters, hk::kKv4Counters, dev, "counters"), (int)sms};
   const c10::cuda::CUDAGuard g(dev);

@@ -74,8 +74,9 @@ struct Kv4Workspace {
   int sms;
 };
 constexpr int kKv4Counters = 2048;  // decode: three per CTA
-// decode: at most 4 CTAs per SM, two partials each of at most 16 heads x (128 + 4) or 8 x (256 + 4)
-constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * 4 * 2 * 2112; }
+// decode: one CTA per SM, with two partials of its own and one of each of its 15 warps (11 where a partial is
+// larger), of at most 16 heads x (128 + 4) or 8 x (256 + 4) floats
+constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * (2 * 2112 + 11 * 2112); }
 
 void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl);
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl);

@@ -24,6 +24,8 @@
 // in one part is written out by its warp; one that spans warps is merged in shared memory at the end
 // of the CTA; one that spans CTAs leaves partials (reference, sum, output), merged in CTA order by the
 // last CTA to arrive (groups of kTree CTAs first, where there are many).
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "sm100.cuh"
 
@@ -33,8 +35,10 @@ namespace {
 using kv4::Unit;
 using sm100::smem_u32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kStages = 2;     // tiles in a warp's ring
-constexpr int kTree = 8;       // CTAs whose partials are merged first
+constexpr int kTree = 8;       // CTAs whose partials are merged first where a pair has more than kFlat
+constexpr int kFlat = 24;
+constexpr int kMinUnits = 8;   // units (and visits) of a warp below which fewer work
+constexpr int kVisit = 4;      // what a pair costs a warp besides its units, in units
 constexpr float kHead = 7.f;   // log2 of how far a score may exceed the reference
 
 __device__ __forceinline__ float ex2(float x) {
@@ -74,11 +78,23 @@ __device__ __forceinline__ uint32_t centre_odd(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Loads past the L1 cache, of shared or global memory, that may be in flight together.
+__device__ __forceinline__ float2 fresh2(const float* p) {
+  float2 v;
+  asm volatile("ld.relaxed.gpu.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 fresh4(const float* p) {
+  float4 v;
+  asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
 struct DecodeArgs {
   Kv4AttnArgs a;
-  int heads_per_item, splits;  // query heads of one item, items per kv head
+  int heads_per_item, split;   // query heads of one item, log2 of the items per kv head (0 or 1)
   int upb_shift;               // log2 of the units per block, or -1
-  float* part;                 // [grid][2][heads_per_item * (HD + 4)]
+  float* part;                 // [grid][2 + kWarps][heads_per_item * (HD + 4)]: the CTAs', then the warps' first
   int* counters;               // [3 * grid], zero between launches
 };
 
@@ -86,190 +102,305 @@ constexpr int kMaxRows = 512;  // rows of one launch
 
 template <int HD, int NT>
 struct DecodeShape {
-  static constexpr int kWarps = NT == 1 && HD <= 128 ? 8 : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kPerSm = NT == 1 && HD <= 128 ? 2 : HD * NT <= 256 ? 3 : 2;  // CTAs, by registers
+  // one CTA per SM (fewer partials to merge than several smaller ones), its warps by the registers:
+  // 128 a thread, or 168
+  static constexpr int kWarps = NT == 1 && HD <= 128 ? 15 : 11;  // and one that issues the copies
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static_assert(2 * kWarps <= 32, "one lane per partial");
+  static constexpr int kStages = NT == 1 && HD <= 128 ? 3 : 4;                     // tiles in a warp's ring
   static constexpr int kTile = 256 / HD;                                           // units per stage (4608 bytes)
   static constexpr int kStageBytes = kTile * Unit<HD>::kBytes;
   static constexpr int kRow = HD + 4;  // floats of one head's partial: output, reference, sum
   static constexpr int kRing = kStages * kStageBytes;
-  // per warp: the ring (whose place the part's last partial takes) and the first partial
-  static size_t warp_bytes(int heads) { return kRing + (size_t)heads * kRow * 4; }
-  static size_t smem(int heads) { return kWarps * warp_bytes(heads); }
+  static constexpr int kSmem = kWarps * kRing;  // the ring's place takes the part's last partial
+  static_assert(kSmem + 10 * 1024 <= 227 * 1024, "shared memory of an SM");
   static_assert(8 * NT * kRow * 4 <= kRing, "the last partial fits the ring");
 };
 
-// One partial of a pair: the CTA's own in shared memory, a CTA's in global memory.
+// A warp's partial in shared memory: units [u0, u1) of a pair.
 struct Part {
   int row, item, u0, u1;  // row < 0: none
 };
 
+// Partials in shared or global memory: number k, i = k + first, at (i % 2 ? odd : even) + (i / 2) stride, in
+// floats, the first one `lead` further on; bit k % 32 of live says whether there is one.
+struct PartList {
+  const float *even, *odd;
+  int first, even_stride, odd_stride, lead;
+  unsigned live;
+};
+
+// Four dims d .. d + 3 of head h of the sum of n partials: to the output of the row's query head `head`
+// (with its sink), or to dst with the references and sums at ml_out (elsewhere than at ml_in if dst is
+// among the partials: other threads may still read those). Out of line: called in two places, runs cold.
+template <int HD>
+__device__ __noinline__ void merge_parts(const Kv4AttnArgs& a, const PartList from, int n, int row, int head, int h,
+                                         int d, int ml_in, float* dst, int ml_out) {
+  constexpr int kRow = HD + 4, kFly = 12;  // loads in flight
+  float m = !dst && a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
+  float lt = m > -INFINITY ? 1.f : 0.f;  // the sink's weight at reference m
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += kFly) {
+    float2 ml[kFly];
+    float4 t[kFly];
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      t[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int i = k0 + k + from.first;
+      if (k0 + k < n && (from.live >> ((k0 + k) & 31) & 1)) {
+        const float* q = (i & 1 ? from.odd + (int64_t)(i >> 1) * from.odd_stride
+                                : from.even + (int64_t)(i >> 1) * from.even_stride) +
+                         (k0 + k ? 0 : from.lead) + h * kRow;
+        ml[k] = fresh2(q + ml_in);
+        t[k] = fresh4(q + d);
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) top = fmaxf(top, ml[k].x);
+    const float mb = fmaxf(top, -1e30f), f = ex2(m - mb);
+    m = top;
+    lt *= f;
+    v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      const float e = ex2(ml[k].x - mb);
+      v.x = fmaf(t[k].x, e, v.x), v.y = fmaf(t[k].y, e, v.y), v.z = fmaf(t[k].z, e, v.z), v.w = fmaf(t[k].w, e, v.w);
+      lt = fmaf(ml[k].y, e, lt);
+    }
+  }
+  if (dst) {
+    __stcg(reinterpret_cast<float4*>(dst + h * kRow + d), v);
+    if (d == 0) __stcg(reinterpret_cast<float2*>(dst + h * kRow + ml_out), make_float2(m, lt));
+    return;
+  }
+  const float f = 1.f / lt;
+  v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+  const int64_t at = (int64_t)head * HD + d;
+  if (a.out_bf16) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(a.out_bf16 + row * a.out_stride + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
+  if (a.out) *reinterpret_cast<float4*>(a.out + row * a.outf_stride + at) = v;
+}
+
 template <int HD, int NT>
-__global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD, NT>::kPerSm)
-    kv4_decode_kernel(DecodeArgs g_) {
+__global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
+    kv4_decode_kernel(const __grid_constant__ DecodeArgs g_) {
   using U = Unit<HD>;
   using Sh = DecodeShape<HD, NT>;
-  constexpr int GR = HD / 64, KT = HD / 16, TU = Sh::kTile, kWarps = Sh::kWarps, kThreads = Sh::kThreads;
-  constexpr int kMinUnits = kWarps;
+  constexpr int GR = HD / 64, KT = HD / 16, TU = Sh::kTile, kWarps = Sh::kWarps, kThreads = Sh::kThreads,
+                kStages = Sh::kStages;
   const Kv4AttnArgs& a = g_.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kWarps][kStages];
-  __shared__ long long before[kMaxRows + 1];  // units of the rows before each row
-  __shared__ long long wsum[kWarps];
+  __shared__ __align__(8) uint64_t full[kWarps][kStages], empty[kWarps][kStages];
+  __shared__ int before[kMaxRows + 1];  // work (units x items) of the rows before each row
+  __shared__ int2 rows[kMaxRows];        // block-table row and context of each row
+  __shared__ int wsum[kWarps + 1];
   __shared__ Part parts[2 * kWarps];
-  __shared__ int last_s;
+  __shared__ int last_s[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int fg = lane >> 2, ft = lane & 3;
-  const int G = a.nh / a.nkv, items = a.nkv * g_.splits, HPI = g_.heads_per_item;
+  const int G = a.nh / a.nkv, items = a.nkv << g_.split, HPI = g_.heads_per_item;
   const int upb = a.block_size / 16;
-  const int wbytes = Sh::kRing + HPI * Sh::kRow * 4;
-  uint8_t* ring = smem + warp * wbytes;
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
+  uint8_t* ring = smem + warp * Sh::kRing;
+  // query heads of an item
+  const auto head_of = [&](int item) { return (item >> g_.split) * G + (item & g_.split) * HPI; };
+  const auto heads_of = [&](int item) { return min(HPI, G - (item & g_.split) * HPI); };
+  if (warp == kWarps && lane < kWarps) {
+    for (int s = 0; s < kStages; ++s) {
+      sm100::mbar_init(&full[lane][s], 1);
+      sm100::mbar_init(&empty[lane][s], 1);
+    }
     sm100::fence_barrier_init();
-    parts[2 * warp].row = parts[2 * warp + 1].row = -1;
+    parts[2 * lane].row = parts[2 * lane + 1].row = -1;
   }
   pdl_wait();
 
-  // ---- work: scan of the rows' units ----
-  const auto row_len = [&](int r, bool report) {
-    const int seq = a.row_seq[r], ctx = a.row_ctx[r];
-    if (seq < 0 || seq >= a.table_rows) {
-      if (report) set_error(a.status, HK_ERR_BAD_ARG);
-      return 0;
-    }
-    return min(max(ctx, 0), a.max_blocks * a.block_size);
-  };
+  // ---- work: scan of the rows' units (the host sees to it that the sum fits 32 bits) ----
   {
     const int per = (a.R + kThreads - 1) / kThreads;
     const int r0 = min(a.R, tid * per), r1 = min(a.R, r0 + per);
-    long long sum = 0;
+    int sum = 0;
+#pragma unroll 1
     for (int r = r0; r < r1; ++r) {
-      const int n = (row_len(r, blockIdx.x == 0) + 15) >> 4;
+      const int seq = a.row_seq[r];
+      int len = min(max(a.row_ctx[r], 0), a.max_blocks * a.block_size);
+      if (seq < 0 || seq >= a.table_rows) {
+        len = 0;
+        if (blockIdx.x == 0) set_error(a.status, HK_ERR_BAD_ARG);
+      }
+      rows[r] = make_int2(seq, len);
+      const int n = len ? (((len + 15) >> 4) + kVisit) * items : 0;
       before[r + 1] = n;
       sum += n;
     }
-    long long inc = sum;
+    int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     if (lane == 31) wsum[warp] = inc;
     if (tid == 0) before[0] = 0;
     __syncthreads();
-    long long base = inc - sum;
+    int base = inc - sum;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
       if (w < warp) base += wsum[w];
+#pragma unroll 1
     for (int r = r0; r < r1; ++r) {
       base += before[r + 1];
       before[r + 1] = base;
     }
     __syncthreads();
   }
-  const long long total = before[a.R] * items;
-  const int N = (int)min((long long)gridDim.x, max(1ll, (total + kMinUnits - 1) / kMinUnits));
+  const int total = before[a.R];
+  // CTAs and warps at work: with few units every SM gets some before its warps multiply
+  const int W = min(kWarps, max(1, (total + (int)gridDim.x * kMinUnits - 1) / ((int)gridDim.x * kMinUnits)));
+  const int N = min((int)gridDim.x, (total + W * kMinUnits - 1) / (W * kMinUnits));
   const int cta = blockIdx.x;
   // rows without context
+#pragma unroll 1
   for (int r = cta; r < a.R; r += gridDim.x)
-    if (before[r + 1] == before[r])
+    if (rows[r].y == 0)
+#pragma unroll 1
       for (int i = tid; i < a.nh * HD; i += kThreads) {
         if (a.out_bf16) a.out_bf16[r * a.out_stride + i] = 0;
         if (a.out) a.out[r * a.outf_stride + i] = 0.f;
       }
-  if (cta >= N || total == 0) return;
-  const long long w0 = total * cta / N, w1 = total * (cta + 1) / N;
-  const long long p0 = w0 + (w1 - w0) * warp / kWarps, p1 = w0 + (w1 - w0) * (warp + 1) / kWarps;
+  if (cta >= N) return;
+  // part i of N * W begins at i * each + min(i, more)
+  const int each = total / (N * W), more = total - each * (N * W);
+  const auto part_begin = [&](int i) { return i * each + min(i, more); };
+  const auto part_of = [&](int x) { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; };
+  const int w0 = part_begin(cta * W);
+  // a warp has its part; in the copying warp lane w has warp w's
+  const bool copies = warp == kWarps;
+  const int who = copies ? lane : warp;
+  const int p0 = part_begin(cta * W + min(who, W)), p1 = part_begin(cta * W + min(who + 1, W));
 
-  // ---- cursor over the pairs of this warp's part [p0, p1) ----
+  // ---- cursor over the pairs of the part [p0, p1) ----
   struct Cursor {
     int row, item, u, units;
-    long long left;  // units of the part still to come
+    int at;  // place of the pair's unit 0: units [u, min(units, p1 - at)) are this part's
   };
   Cursor cc;
   {
-    int lo = 0, hi = a.R;  // last row with before * items <= p0
+    int lo = 0, hi = a.R;  // last row with before <= p0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (before[mid] * items <= p0) lo = mid;
+      if (before[mid] <= p0) lo = mid;
       else hi = mid;
     }
     cc.row = lo;
-    cc.units = (int)(before[lo + 1] - before[lo]);
-    const long long off = p0 - before[lo] * items;
-    cc.item = cc.units ? (int)(off / cc.units) : 0;
-    cc.u = (int)(off - (long long)cc.item * cc.units);
-    cc.left = p1 - p0;
+    cc.units = (rows[lo].y + 15) >> 4;
+    cc.item = cc.units ? (p0 - before[lo]) / (cc.units + kVisit) : 0;
+    cc.at = before[lo] + cc.item * (cc.units + kVisit) + kVisit;
+    cc.u = max(0, p0 - cc.at);
   }
-  const auto next_pair = [&](Cursor& c) {  // only while units are left
+  const auto more_in = [&](const Cursor& c) { return c.at + c.u < p1; };
+  const auto next_pair = [&](Cursor& c) {  // to the next pair (which may lie past the part)
     c.u = 0;
+    c.at += c.units + kVisit;
     if (++c.item == items) {
       c.item = 0;
       do ++c.row;
-      while (before[c.row + 1] == before[c.row]);
-      c.units = (int)(before[c.row + 1] - before[c.row]);
+      while (c.row < a.R && rows[c.row].y == 0);
+      c.units = c.row < a.R ? (rows[c.row].y + 15) >> 4 : 0;
     }
   };
 
-  // ---- producer: the part's tiles in order, kStages ahead ----
-  Cursor pc = cc;
-  int p_stage = 0, blk = 0, pos = 0;  // this lane's block and unit in the block, of the next tile
-  const uint8_t* p_head = nullptr;    // the pair's kv head in block 0
-  const int* p_table = nullptr;
-  const int64_t blk_bytes = (int64_t)a.nkv * upb * U::kBytes;
-  const auto pair_base = [&]() {
-    p_head = a.cache + (int64_t)(pc.item / g_.splits) * upb * U::kBytes;
-    p_table = a.block_tables + (int64_t)a.row_seq[pc.row] * a.max_blocks;
-  };
-  const auto fetch = [&]() {  // block ids of the next tile's units, one per lane
-    const int u = pc.u + lane;
-    if (lane < TU && u < pc.units) {
-      const int b = g_.upb_shift >= 0 ? u >> g_.upb_shift : u / upb;
-      pos = u - b * upb;
-      blk = p_table[b];
-    }
-  };
-  const auto produce = [&]() {
-    if (pc.left <= 0) return;
-    uint8_t* dst = ring + p_stage * Sh::kStageBytes + lane * U::kBytes;
-    uint64_t* bar = &full[warp][p_stage];
-    const int n = (int)min((long long)min(TU, pc.units - pc.u), pc.left);
-    const bool mine = lane < n, good = mine && blk >= 0 && blk < a.cache_blocks;
-    const unsigned m = __ballot_sync(0xffffffffu, good);
-    if (mine && !good) {  // a block outside the cache reads as zeros
-      set_error(a.status, HK_ERR_BAD_ARG);
-      for (int i = 0; i < U::kBytes; i += 16) *reinterpret_cast<uint4*>(dst + i) = make_uint4(0u, 0u, 0u, 0u);
-      sm100::fence_proxy_async_smem();
-    }
-    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, __popc(m) * U::kBytes);
-    __syncwarp();
-    if (good) sm100::bulk_g2s(dst, p_head + blk * blk_bytes + pos * U::kBytes, U::kBytes, bar);
-    p_stage = p_stage + 1 == kStages ? 0 : p_stage + 1;
-    pc.u += n;
-    pc.left -= n;
-    if (pc.left > 0) {
-      if (pc.u == pc.units) {
-        next_pair(pc);
-        pair_base();
+  // ---- the copying warp: every lane fetches one warp's tiles, kStages ahead, so that the cursors and
+  // addresses of all warps cost one warp's instructions ----
+  if (copies) {
+    const uint8_t* head = nullptr;  // the pair's kv head in block 0
+    const int* table = nullptr;
+    const int64_t blk_bytes = (int64_t)a.nkv * upb * U::kBytes;
+    int blk_last = 0;  // block of the last tile's last unit
+    int blk[TU], at = 0;  // blocks of the next tile's units, and the first unit's place in its block
+    const auto lookup = [&](bool pair) {
+      if (pair) {
+        head = a.cache + (int64_t)(cc.item >> g_.split) * upb * U::kBytes;
+        table = a.block_tables + (int64_t)rows[cc.row].x * a.max_blocks;
       }
-      fetch();
-    }
-  };
-  if (pc.left > 0) {
-    pair_base();
-    fetch();
-  }
+      const int b0 = g_.upb_shift >= 0 ? cc.u >> g_.upb_shift : cc.u / upb;
+      at = cc.u - b0 * upb;
+      const bool kept = !pair && at > 0;  // the tile begins in the last one's block
+      int b = b0, k = at;
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) produce();
+      for (int i = 0; i < TU; ++i) {
+        if (i > 0 && ++k == upb) k = 0, ++b;
+        if (i == 0 && kept) blk[0] = blk_last;
+        else if (i > 0 && b == b0) blk[i] = blk[0];
+        else if (cc.u + i < cc.units) blk[i] = table[b];
+      }
+    };
+    uint8_t* const my_ring = smem + lane * Sh::kRing;
+    int st = 0, ph = 1;
+    bool more = lane < W && more_in(cc);
+    if (more) lookup(true);
+#pragma unroll 1
+    for (unsigned spin = 0; __any_sync(0xffffffffu, more); ++spin) {
+      const bool go = more && sm100::mbar_try_wait(&empty[lane][st], ph);
+      if (go) {
+        const int n = min(TU, min(cc.units, p1 - cc.at) - cc.u);
+        uint8_t* dst = my_ring + st * Sh::kStageBytes;
+        uint64_t* bar = &full[lane][st];
+        int good = 0;
+#pragma unroll
+        for (int i = 0; i < TU; ++i) {
+          if (i < n) {
+            if (blk[i] >= 0 && blk[i] < a.cache_blocks) {
+              ++good;
+            } else {  // a block outside the cache reads as zeros
+              set_error(a.status, HK_ERR_BAD_ARG);
+#pragma unroll 1
+              for (int x = 0; x < U::kBytes; x += 16)
+                *reinterpret_cast<uint4*>(dst + i * U::kBytes + x) = make_uint4(0u, 0u, 0u, 0u);
+              sm100::fence_proxy_async_smem();
+            }
+            blk_last = blk[i];
+          }
+        }
+        sm100::mbar_arrive_expect_tx(bar, good * U::kBytes);
+        int k = at;  // one copy for the units of one block
+#pragma unroll
+        for (int i = 0; i < TU; ++i) {
+          if (i < n && (i == 0 || k == 0) && blk[i] >= 0 && blk[i] < a.cache_blocks)
+            sm100::bulk_g2s(dst + i * U::kBytes, head + blk[i] * blk_bytes + k * U::kBytes,
+                            min(n - i, upb - k) * U::kBytes, bar);
+          if (++k == upb) k = 0;
+        }
+        if (++st == kStages) st = 0, ph ^= 1;
+        cc.u += n;
+        const bool pair = cc.u == cc.units;
+        if (pair) next_pair(cc);
+        more = more_in(cc);
+        if (more) lookup(pair);
+        spin = 0;
+      }
+      if (!__any_sync(0xffffffffu, go)) {
+        if (spin > (1u << 24)) {  // warps that never free a stage
+          set_error(a.status, HK_ERR_MBAR_TIMEOUT);
+          break;
+        }
+        __nanosleep(64);
+      }
+    }
+  }
 
-  // ---- consumer ----
+  // ---- the other warps: one pair after the other. A pair's part goes out (if it is the whole pair) or to a
+  // partial: the first of the warp's to global memory (its ring is in use), the last to the ring's place ----
+  const int pstride = HPI * Sh::kRow;
+  float* const firsts = g_.part + ((int64_t)gridDim.x * 2 + (int64_t)cta * kWarps) * pstride;
   int c_stage = 0, c_phase = 0;
-  bool first_pair = true;
-  while (cc.left > 0) {
-    const int u_first = cc.u, kvh = cc.item / g_.splits, h0 = kvh * G + (cc.item % g_.splits) * HPI;
-    const int heads = min(HPI, kvh * G + G - h0);
-    const int len = row_len(cc.row, false);
+  while (!copies && more_in(cc)) {
+    const int u_first = cc.u, h0 = head_of(cc.item), heads = heads_of(cc.item);
+    const int len = rows[cc.row].y;
     // queries: B fragments (dims x 8 heads), float16 after a power-of-two scaling of each head
     uint32_t qf[NT][KT][2];
     float mult[NT][2], qsum[NT][2][GR];
@@ -283,34 +414,36 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
         if (h < heads)
           raw[i] = *reinterpret_cast<const uint4*>(a.q + cc.row * a.q_stride + (int64_t)(h0 + h) * HD + 32 * i + 8 * ft);
       }
-      float mx = 0.f, qs[GR];
+      __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
+      }
+      float mx = fmaxf(__low2float(top), __high2float(top));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^-e with 1 <= mx 2^-e < 2 (1 for a zero, subnormal or non-finite head), exact in bf16
+      const int ex = (int)(__float_as_uint(mx) >> 23);
+      const bool norm = ex > 4 && ex < 254;
+      const uint32_t dn = norm ? (uint32_t)(254 - ex) << 7 : 0x3f80u, dn16 = dn + (4u << 7);
+      const uint32_t d1 = dn | dn << 16, d16 = dn16 | dn16 << 16;
+      // 2^24 of the subnormal codes, less the 16 of the query
+      const float un = norm ? __uint_as_float((uint32_t)ex << 23) : 1.f, up = un * (a.scale * kLog2e * 1048576.f);
+      float qs[GR];
 #pragma unroll
       for (int grp = 0; grp < GR; ++grp) qs[grp] = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lo = __uint_as_float(w[j] << 16), hi = __uint_as_float(w[j] & 0xffff0000u);
-          mx = fmaxf(mx, fmaxf(fabsf(lo), fabsf(hi)));
-          qs[i / 2] += lo + hi;
-        }
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // 2^-e with 1 <= mx 2^-e < 2 (1 for a zero, subnormal or non-finite head)
-      const int ex = (int)(__float_as_uint(mx) >> 23);
-      const float down = ex > 0 && ex < 254 ? __uint_as_float((uint32_t)(254 - ex) << 23) : 1.f;
-      // 2^24 of the subnormal codes, less the 16 of the query
-      const float up = (ex > 0 && ex < 254 ? __uint_as_float((uint32_t)ex << 23) : 1.f) * (a.scale * kLog2e * 1048576.f);
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lo = __uint_as_float(w[j] << 16) * down, hi = __uint_as_float(w[j] & 0xffff0000u) * down;
-          const float f = j & 1 ? 1.f : 16.f;  // the odd nibbles' codes come 16 times larger
-          qf[nt][2 * i + j / 2][j & 1] = pack_f16(lo * f, hi * f);
+        for (int j = 0; j < 4; ++j) {  // the odd nibbles' codes come 16 times larger
+          const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]),
+                                           *reinterpret_cast<const __nv_bfloat162*>(j & 1 ? &d1 : &d16));
+          const float lo = __low2float(y), hi = __high2float(y);
+          qf[nt][2 * i + j / 2][j & 1] = pack_f16(lo, hi);
+          qs[i / 2] = fmaf(lo + hi, j & 1 ? 1.f : 0.0625f, qs[i / 2]);
         }
       }
 #pragma unroll
@@ -323,7 +456,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
         mult[nt][c] = __shfl_sync(0xffffffffu, up, (2 * ft + c) * 4);
 #pragma unroll
         for (int grp = 0; grp < GR; ++grp)
-          qsum[nt][c][grp] = __shfl_sync(0xffffffffu, qs[grp], (2 * ft + c) * 4) * a.scale * kLog2e;
+          qsum[nt][c][grp] = __shfl_sync(0xffffffffu, qs[grp] * un, (2 * ft + c) * 4) * (a.scale * kLog2e);
       }
     }
     float o[NT][KT][4], ref[NT][2], l[NT][2], oc[NT][2][GR];
@@ -333,15 +466,17 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
       for (int m = 0; m < KT; ++m) o[nt][m][0] = o[nt][m][1] = o[nt][m][2] = o[nt][m][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        ref[nt][c] = -INFINITY;
+        ref[nt][c] = 0.f;
         l[nt][c] = 0.f;
 #pragma unroll
         for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] = 0.f;
       }
     }
-    float sdown = 16777216.f;  // 2^-E
-    while (cc.left > 0 && cc.u < cc.units) {
-      const int n = (int)min((long long)min(TU, cc.units - cc.u), cc.left);
+    float log2_s = -24.f;  // E
+    bool first = true;     // no reference yet
+    const int u_last = min(cc.units, p1 - cc.at);
+    while (cc.u < u_last) {
+      const int n = min(TU, u_last - cc.u);
       const uint8_t* base = ring + c_stage * Sh::kStageBytes;
       sm100::mbar_wait(&full[warp][c_stage], c_phase, a.status);
       float s[TU][NT][4];
@@ -349,7 +484,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
       // scores and value pairs of the tile
 #pragma unroll
       for (int j = 0; j < TU; ++j) {
-        if (j < n) {
+        {
           const uint8_t* un = base + j * U::kBytes;
           float acc[NT][GR][4];
 #pragma unroll
@@ -396,7 +531,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                   x[nt][c] = grp ? fmaf(p.x, acc[nt][grp][2 * half + c], x[nt][c]) : p.x * acc[nt][grp][2 * half + c];
-                  y[nt][c] = grp ? fmaf(b, qsum[nt][c][grp], y[nt][c]) : b * qsum[nt][c][grp];
+                  y[nt][c] = fmaf(b, qsum[nt][c][grp], grp ? y[nt][c] : -ref[nt][c]);
                 }
             }
 #pragma unroll
@@ -404,23 +539,15 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
 #pragma unroll
               for (int c = 0; c < 2; ++c) s[j][nt][2 * half + c] = fmaf(x[nt][c], mult[nt][c], y[nt][c]);
           }
-        } else {
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int grp = 0; grp < GR; ++grp) vp[j][half][grp] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][nt][e] = -INFINITY;
         }
       }
-      if ((cc.u + n) * 16 > len) {  // the last unit's tokens past the context hold stale bytes: whatever they are
+      const int lim = min(len, (cc.u + n) * 16);
+      if (lim < (cc.u + TU) * 16) {  // past the tile or the context: stale bytes, whatever they hold
 #pragma unroll
         for (int j = 0; j < TU; ++j)
 #pragma unroll
           for (int half = 0; half < 2; ++half)
-            if ((cc.u + j) * 16 + fg + 8 * half >= len) {
+            if ((cc.u + j) * 16 + fg + 8 * half >= lim) {
 #pragma unroll
               for (int grp = 0; grp < GR; ++grp) vp[j][half][grp] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
@@ -439,7 +566,8 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
             for (int grp = 0; grp < GR; ++grp) t = __hmax2(t, __habs2(vp[j][half][grp]));
         top_s = __low2float(t);
       }
-      bool move = top_s * sdown > 1.f;
+      const float bound = kHead - log2_s;  // scores are relative to ref = R + E
+      bool move = first || top_s > ex2(log2_s);
       float mx[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -448,52 +576,54 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
           mx[nt][c] = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
 #pragma unroll
           for (int j = 1; j < TU; ++j) mx[nt][c] = fmaxf(mx[nt][c], fmaxf(s[j][nt][c], s[j][nt][2 + c]));
-          move |= mx[nt][c] > ref[nt][c] + kHead;
+          move |= mx[nt][c] > bound;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, off));
-        // 2^-E with E the exponent above the largest scale so far
-        const float need = top_s > 0.f ? __uint_as_float((uint32_t)(253 - (int)(__float_as_uint(top_s) >> 23)) << 23) : sdown;
-        const float nd = fminf(sdown, need), fall = nd / sdown;
-        sdown = nd;
+        // E: at least the exponent above the largest scale so far
+        const float e_new = fmaxf(log2_s, (float)((int)(__float_as_uint(top_s) >> 23) - 126));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float m = fmaxf(ref[nt][c], mx[nt][c]);
+            float m = mx[nt][c];
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-            const float corr = m > -INFINITY ? ex2(ref[nt][c] - m) : 1.f;
-            ref[nt][c] = m;
+            m += log2_s;  // the tile's largest score, relative to R
+            const float rise = m > -INFINITY && (first || m > 0.f) ? m : 0.f;
+            const float up_to = rise + (e_new - log2_s), corr = first ? 1.f : ex2(-up_to);
+            ref[nt][c] += up_to;
             l[nt][c] *= corr;
 #pragma unroll
             for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] *= corr;
-            const float f = corr * fall;
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
-              o[nt][k][c] *= f;
-              o[nt][k][2 + c] *= f;
+              o[nt][k][c] *= corr;
+              o[nt][k][2 + c] *= corr;
             }
+#pragma unroll
+            for (int j = 0; j < TU; ++j) s[j][nt][c] -= up_to, s[j][nt][2 + c] -= up_to;
           }
+        log2_s = e_new;
+        first = false;
       }
       // weights and values
 #pragma unroll
       for (int j = 0; j < TU; ++j) {
-        if (j < n) {
+        {
           uint32_t pb[NT][GR][2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float sv[GR], vc[GR];
 #pragma unroll
             for (int grp = 0; grp < GR; ++grp) {
-              sv[grp] = __low2float(vp[j][half][grp]) * sdown;
+              sv[grp] = __low2float(vp[j][half][grp]);
               vc[grp] = __high2float(vp[j][half][grp]);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float w0_ = ex2(s[j][nt][2 * half] - fmaxf(ref[nt][0], -1e30f));
-              const float w1_ = ex2(s[j][nt][2 * half + 1] - fmaxf(ref[nt][1], -1e30f));
+              const float w0_ = ex2(s[j][nt][2 * half]), w1_ = ex2(s[j][nt][2 * half + 1]);
               l[nt][0] += w0_;
               l[nt][1] += w1_;
 #pragma unroll
@@ -524,189 +654,152 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
         }
       }
       cc.u += n;
-      cc.left -= n;
-      if (++c_stage == kStages) c_stage = 0, c_phase ^= 1;
       __syncwarp();
-      produce();  // into the stage whose last operands the instructions above have taken
+      if (lane == 0) sm100::mbar_arrive(&empty[warp][c_stage]);
+      if (++c_stage == kStages) c_stage = 0, c_phase ^= 1;
     }
 
     // ---- the pair's result in this part ----
-    const float sup = 1.f / sdown;
     const bool whole = u_first == 0 && cc.u == cc.units;
-    const int slot = first_pair ? 0 : 1;
-    float* dst0 = reinterpret_cast<float*>(ring + (slot ? 0 : Sh::kRing));
+    const int slot = cc.at + cc.units + kVisit >= p1 ? 1 : 0;  // the part's last pair: its ring is done
+    float* mine = slot ? reinterpret_cast<float*>(ring) : firsts + warp * pstride;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int h = nt * 8 + 2 * ft + c;
+        float lt = l[nt][c], f = 1.f;
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
-          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+          lt += __shfl_xor_sync(0xffffffffu, lt, off);
 #pragma unroll
           for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] += __shfl_xor_sync(0xffffffffu, oc[nt][c][grp], off);
         }
         if (h < heads) {
-          float f = 1.f;
+          float* to = mine + h * Sh::kRow + 4 * fg;  // fp32: the partial, or the output itself
+          uint16_t* to16 = nullptr;
           if (whole) {
-            float lt = l[nt][c], e = 1.f;
-            if (a.sinks) {
-              const float sk = a.sinks[h0 + h] * kLog2e, m = fmaxf(sk, ref[nt][c]), mb = fmaxf(m, -1e30f);
-              e = ex2(ref[nt][c] - mb);
-              lt = fmaf(lt, e, ex2(sk - mb));
-            }
-            f = e / lt;
+            const int64_t at = (int64_t)(h0 + h) * HD + 4 * fg;
+            if (a.sinks) lt += ex2(fminf(a.sinks[h0 + h] * kLog2e - ref[nt][c], 126.f));
+            f = __frcp_rn(lt);
+            to = a.out ? a.out + cc.row * a.outf_stride + at : nullptr;
+            to16 = a.out_bf16 ? a.out_bf16 + cc.row * a.out_stride + at : nullptr;
+          } else if (fg == 0) {
+            *reinterpret_cast<float2*>(mine + h * Sh::kRow + HD) = make_float2(ref[nt][c], lt);
           }
 #pragma unroll
           for (int k = 0; k < KT; k += 2) {
-            const int d = (k >> 2) * 64 + ((k >> 1) & 1) * 32 + 4 * fg;
-            float4 v = make_float4(fmaf(o[nt][k][c], sup, oc[nt][c][k >> 2]), fmaf(o[nt][k][2 + c], sup, oc[nt][c][k >> 2]),
-                                   fmaf(o[nt][k + 1][c], sup, oc[nt][c][k >> 2]),
-                                   fmaf(o[nt][k + 1][2 + c], sup, oc[nt][c][k >> 2]));
-            if (whole) {
-              v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-              const int64_t at = (int64_t)(h0 + h) * HD + d;
-              if (a.out_bf16) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-                *reinterpret_cast<uint2*>(a.out_bf16 + cc.row * a.out_stride + at) =
-                    make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-              }
-              if (a.out) *reinterpret_cast<float4*>(a.out + cc.row * a.outf_stride + at) = v;
-            } else {
-              *reinterpret_cast<float4*>(dst0 + h * Sh::kRow + d) = v;
+            const int d = (k >> 2) * 64 + ((k >> 1) & 1) * 32;
+            const float z = oc[nt][c][k >> 2];
+            const float4 v = make_float4((o[nt][k][c] + z) * f, (o[nt][k][2 + c] + z) * f, (o[nt][k + 1][c] + z) * f,
+                                         (o[nt][k + 1][2 + c] + z) * f);
+            if (to) *reinterpret_cast<float4*>(to + d) = v;
+            if (to16) {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+              *reinterpret_cast<uint2*>(to16 + d) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
             }
-          }
-          if (!whole && fg == 0) {
-            dst0[h * Sh::kRow + HD] = ref[nt][c];
-            dst0[h * Sh::kRow + HD + 1] = l[nt][c];
           }
         }
       }
     if (!whole && lane == 0) parts[2 * warp + slot] = Part{cc.row, cc.item, u_first, cc.u};
-    first_pair = false;
-    if (cc.left > 0) next_pair(cc);
+    next_pair(cc);
   }
 
-  // ---- pairs that span warps or CTAs ----
+  // ---- pairs that span warps or CTAs (rolled loops: this code runs once per CTA, cold) ----
   __syncthreads();
-  const int pstride = HPI * Sh::kRow;
-  const auto local = [&](int i) {  // partial i of the CTA
-    return reinterpret_cast<const float*>(smem + (i >> 1) * wbytes + (i & 1 ? 0 : Sh::kRing));
-  };
-  const auto emit4 = [&](int row, int h, int d, float4 v, float f) {
-    v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-    if (a.out_bf16) {
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-      *reinterpret_cast<uint2*>(a.out_bf16 + row * a.out_stride + (int64_t)h * HD + d) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    }
-    if (a.out) *reinterpret_cast<float4*>(a.out + row * a.outf_stride + (int64_t)h * HD + d) = v;
-  };
-  const auto sink_of = [&](int h) { return a.sinks ? a.sinks[h] * kLog2e : -INFINITY; };
-  for (int i = 0; i < 2 * kWarps;) {
-    const Part p = parts[i];
-    if (p.row < 0) {
-      ++i;
-      continue;
-    }
-    unsigned set = 0;  // the pair's partials in this CTA
-    int end = p.u1, j = i;
-    for (; j < 2 * kWarps; ++j) {
-      const Part q = parts[j];
-      if (q.row < 0) continue;
-      if (q.row != p.row || q.item != p.item) break;
-      set |= 1u << j;
-      end = q.u1;
-    }
-    i = j;
-    const int units = (int)(before[p.row + 1] - before[p.row]);
-    const bool done = p.u0 == 0 && end == units;
-    const long long i0 = before[p.row] * items + (long long)p.item * units, i1 = i0 + units;
-    const int kvh = p.item / g_.splits, h0 = kvh * G + (p.item % g_.splits) * HPI;
-    const int heads = min(HPI, kvh * G + G - h0);
-    const int my_slot = i0 + p.u0 == w0 ? 0 : 1;
-    float* mine = g_.part + ((int64_t)cta * 2 + my_slot) * pstride;
-    for (int x = tid; x < heads * (HD / 4); x += kThreads) {
-      const int h = x / (HD / 4), d = x % (HD / 4) * 4;
-      const float sk = done ? sink_of(h0 + h) : -INFINITY;
-      float m = sk;
-      for (unsigned b = set; b; b &= b - 1) m = fmaxf(m, local(__ffs(b) - 1)[h * Sh::kRow + HD]);
-      const float mb = fmaxf(m, -1e30f);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float lt = ex2(sk - mb);
-      for (unsigned b = set; b; b &= b - 1) {
-        const float* q = local(__ffs(b) - 1) + h * Sh::kRow;
-        const float e = ex2(q[HD] - mb);
-        const float4 t = *reinterpret_cast<const float4*>(q + d);
-        v.x = fmaf(t.x, e, v.x), v.y = fmaf(t.y, e, v.y), v.z = fmaf(t.z, e, v.z), v.w = fmaf(t.w, e, v.w);
-        lt = fmaf(q[HD + 1], e, lt);
-      }
-      if (done) {
-        emit4(p.row, h0 + h, d, v, 1.f / lt);
-      } else {
-        __stcg(reinterpret_cast<float4*>(mine + h * Sh::kRow + d), v);
-        if (d == 0) __stcg(reinterpret_cast<float2*>(mine + h * Sh::kRow + HD), make_float2(m, lt));
+  // the CTA's pairs that reach into others: at most one at its begin (0) and one at its end (1)
+  __shared__ int span[2][5];  // row (-1: none), item, CTAs c0 .. c1, slot of c0's partial (the others' are 0)
+  if (tid < 2) span[tid][0] = -1;
+  __syncthreads();
+  {
+    const Part p = lane < 2 * kWarps ? parts[lane] : Part{-1, 0, 0, 0};
+    const unsigned valid = __ballot_sync(0xffffffffu, p.row >= 0);
+    const unsigned below = valid & ((1u << lane) - 1);
+    const int prev = below ? 31 - __clz(below) : lane;
+    const int prow = __shfl_sync(0xffffffffu, p.row, prev), pitem = __shfl_sync(0xffffffffu, p.item, prev);
+    const unsigned begins = __ballot_sync(0xffffffffu, p.row >= 0 && (!below || prow != p.row || pitem != p.item));
+    // all pairs at once: item x is four dims of one head of pair x / per
+    const int per = HPI * (HD / 4), work = __popc(begins) * per;
+#pragma unroll 1
+    for (int x = tid; x < work; x += kThreads) {
+      unsigned left = begins;
+#pragma unroll 1
+      for (int g = x / per; g > 0; --g) left &= left - 1;
+      const int i0 = __ffs(left) - 1;
+      const unsigned rest = left & (left - 1);
+      const unsigned set = valid & ~((1u << i0) - 1) & (rest ? (rest & -rest) - 1 : ~0u);
+      const int i1 = 31 - __clz(set);
+      const Part f = parts[i0];
+      const int u1 = parts[i1].u1, units = (rows[f.row].y + 15) >> 4;
+      const bool done = f.u0 == 0 && u1 == units;
+      const int at0 = before[f.row] + f.item * (units + kVisit) + kVisit;  // place of its unit 0
+      const int slot = at0 + f.u0 <= w0 ? 0 : 1;
+      float* dst = done ? nullptr : g_.part + ((int64_t)cta * 2 + slot) * pstride;
+      const PartList from{firsts, reinterpret_cast<const float*>(smem), i0, pstride, Sh::kRing / 4, 0, set >> i0};
+      const int y = x % per, h = y / (HD / 4), d = y % (HD / 4) * 4;
+      if (h < heads_of(f.item)) merge_parts<HD>(a, from, i1 - i0 + 1, f.row, head_of(f.item) + h, h, d, HD, dst, HD);
+      if (!done && y == 0) {
+        const int c0 = part_of(at0) / W;
+        span[slot][1] = f.item;
+        span[slot][2] = c0;
+        span[slot][3] = part_of(at0 + units - 1) / W;
+        span[slot][4] = part_begin(c0 * W) < at0 ? 1 : 0;
+        span[slot][0] = f.row;
       }
     }
-    if (done) continue;
-    // partials of several CTAs: c0 .. c1 in order, the first of them in slot 1 unless the pair begins it
-    const int c0 = (int)(((i0 + 1) * N - 1) / total), c1 = (int)((i1 * N - 1) / total);
-    const int first_slot = total * c0 / N < i0 ? 1 : 0;
-    const auto part_of = [&](int c) { return g_.part + ((int64_t)c * 2 + (c == c0 ? first_slot : 0)) * pstride; };
-    // true in the last of `n` CTAs to come here (its reads see the others' writes)
-    const auto arrive_last = [&](int* counter, int n) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const int got = atomicAdd(counter, 1);
-        last_s = got == n - 1;
-        if (last_s) *counter = 0;
-      }
-      __syncthreads();
-      const bool last = last_s;
-      __syncthreads();
-      if (last) __threadfence();
-      return last;
-    };
-    // sum of the partials from, from + step, .. < to, to the row's output or to dst (with its reference and
-    // sum two places on: others still read the first). `ml`: where the partials' reference and sum are
-    const auto merge = [&](int from, int to, int step, int ml_at, float* dst) {
-      for (int x = tid; x < heads * (HD / 4); x += kThreads) {
-        const int h = x / (HD / 4), d = x % (HD / 4) * 4;
-        const float sk = dst ? -INFINITY : sink_of(h0 + h);
-        float m = sk;
-#pragma unroll 8
-        for (int c = from; c < to; c += step) m = fmaxf(m, __ldcg(part_of(c) + h * Sh::kRow + ml_at));
-        const float mb = fmaxf(m, -1e30f);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float lt = ex2(sk - mb);
-#pragma unroll 8
-        for (int c = from; c < to; c += step) {
-          const float* q = part_of(c) + h * Sh::kRow;
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + ml_at));
-          const float4 t = __ldcg(reinterpret_cast<const float4*>(q + d));
-          const float e = ex2(ml.x - mb);
-          v.x = fmaf(t.x, e, v.x), v.y = fmaf(t.y, e, v.y), v.z = fmaf(t.z, e, v.z), v.w = fmaf(t.w, e, v.w);
-          lt = fmaf(ml.y, e, lt);
+  }
+  // Round 0: the last CTA of a pair to arrive sums its partials; where there are many, the last of each
+  // kTree CTAs sums theirs, and in round 1 the last of these sums the sums.
+#pragma unroll 1
+  for (int round = 0; round < 2; ++round) {
+    __threadfence();
+    __syncthreads();
+    if (span[0][0] < 0 && span[1][0] < 0) break;
+    if (tid < 2) {
+      int last = 0;
+      const int* sp = span[tid];
+      if (sp[0] >= 0) {
+        const int n = sp[3] - sp[2] + 1, g0 = (cta - sp[2]) / kTree * kTree;
+        const bool deep = n > kFlat;
+        int* counter = g_.counters + sp[2];
+        int want = n;
+        if (deep && round == 0) {
+          counter = g_.counters + gridDim.x + 2 * (sp[2] + g0) + (g0 == 0 ? sp[4] : 0);
+          want = min(kTree, n - g0);
+        } else if (deep) {
+          want = (n + kTree - 1) / kTree;
         }
-        if (dst) {
-          __stcg(reinterpret_cast<float4*>(dst + h * Sh::kRow + d), v);
-          if (d == 0) __stcg(reinterpret_cast<float2*>(dst + h * Sh::kRow + HD + 2), make_float2(m, lt));
-        } else {
-          emit4(p.row, h0 + h, d, v, 1.f / lt);
-        }
+        last = atomicAdd(counter, 1) == want - 1;
+        if (last) *counter = 0;
       }
-    };
-    const int n = c1 - c0 + 1;
-    if (n <= 2 * kTree) {
-      if (arrive_last(g_.counters + c0, n)) merge(c0, c1 + 1, 1, HD, nullptr);
-    } else {
-      const int grp = (cta - c0) / kTree, g0 = c0 + grp * kTree, g1 = min(g0 + kTree, c1 + 1);
-      if (arrive_last(g_.counters + gridDim.x + 2 * g0 + (g0 == c0 ? first_slot : 0), g1 - g0)) {
-        merge(g0, g1, 1, HD, part_of(g0));
-        if (arrive_last(g_.counters + c0, (n + kTree - 1) / kTree)) merge(c0, c1 + 1, kTree, HD + 2, nullptr);
-      }
+      last_s[tid] = last;
     }
+    __syncthreads();
+    __threadfence();
+    bool again = false;
+    const int per = HPI * (HD / 4);
+#pragma unroll 1
+    for (int x = tid; x < 2 * per; x += kThreads) {
+      const int s = x >= per ? 1 : 0;
+      if (!last_s[s]) continue;
+      const int row = span[s][0], item = span[s][1], c0 = span[s][2], n = span[s][3] - c0 + 1, first = span[s][4];
+      const bool deep = n > kFlat, inner = deep && round == 0;
+      const int g0 = inner ? (cta - c0) / kTree * kTree : 0, step = deep && round ? kTree : 1;
+      const int cnt = inner ? min(kTree, n - g0) : deep ? (n + kTree - 1) / kTree : n;
+      float* part = g_.part + (int64_t)(c0 + g0) * 2 * pstride;
+      const int off = g0 == 0 ? first * pstride : 0;
+      const PartList from{part, part + 2 * step * pstride, 0, 4 * step * pstride, 4 * step * pstride, off, ~0u};
+      const int y = x - s * per, h = y / (HD / 4), d = y % (HD / 4) * 4;
+      if (h < heads_of(item))
+        merge_parts<HD>(a, from, cnt, row, head_of(item) + h, h, d, deep && round ? HD + 2 : HD,
+                        inner ? part + off : nullptr, HD + 2);
+    }
+    for (int s = 0; s < 2; ++s) again |= last_s[s] && round == 0 && span[s][3] - span[s][2] + 1 > kFlat;
+    if (!again) break;
+    // only the spans summed in this round arrive in the next
+    __syncthreads();
+    if (tid < 2 && !(last_s[tid] && span[tid][3] - span[tid][2] + 1 > kFlat)) span[tid][0] = -1;
   }
   pdl_launch();
 }
@@ -714,28 +807,27 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, DecodeShape<HD,
 template <int HD, int NT>
 void launch_decode(const DecodeArgs& d, int sms, cudaStream_t s, bool pdl) {
   using Sh = DecodeShape<HD, NT>;
-  const size_t smem = Sh::smem(d.heads_per_item);
-  static int per_sm[8 * NT + 1] = {};  // by heads per item; per instantiation, one device per process
-  int& resident = per_sm[d.heads_per_item];
-  if (!resident) {
+  static bool configured = false;  // per instantiation; one device per process
+  if (!configured) {
     HK_CUDA_CHECK(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)Sh::smem(8 * NT)));
-    int n = 0;
-    HK_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_decode_kernel<HD, NT>, Sh::kThreads, smem));
-    if (n < 1) throw std::runtime_error("kv4 attention decode: the kernel does not fit on an SM");
-    resident = n < 4 ? n : 4;
+                                       Sh::kSmem));
+    configured = true;
   }
-  launch(kv4_decode_kernel<HD, NT>, dim3(sms * resident), dim3(Sh::kThreads), smem, s, pdl, d);
+  launch(kv4_decode_kernel<HD, NT>, dim3(sms), dim3(Sh::kThreads), Sh::kSmem, s, pdl, d);
 }
 
 }  // namespace
 
 void kv4_attention_decode_launch(const Kv4AttnArgs& args, const Kv4Workspace& ws, cudaStream_t s, bool pdl) {
   const int G = args.nh / args.nkv;
-  for (int r0 = 0; r0 < args.R; r0 += kMaxRows) {
+  // rows of a launch: the sum of their units x items stays below 2^31
+  const int64_t most = ((int64_t)args.max_blocks * (args.block_size / 16) + 1) * args.nkv * 2;
+  const int chunk = (int)std::min<int64_t>(kMaxRows, ((int64_t(1) << 31) - 1) / most);
+  if (chunk < 1) throw std::runtime_error("kv4 attention decode: context x kv heads too large");
+  for (int r0 = 0; r0 < args.R; r0 += chunk) {
     DecodeArgs d{};
     d.a = args;
-    d.a.R = args.R - r0 < kMaxRows ? args.R - r0 : kMaxRows;
+    d.a.R = args.R - r0 < chunk ? args.R - r0 : chunk;
     d.a.q += r0 * args.q_stride;
     d.a.row_seq += r0;
     d.a.row_ctx += r0;
@@ -745,7 +837,7 @@ void kv4_attention_decode_launch(const Kv4AttnArgs& args, const Kv4Workspace& ws
     d.counters = ws.counters;
     const bool wide = G > 8 && args.hd <= 128;  // two tiles of 8 heads share each key and value
     d.heads_per_item = wide ? G : (G < 8 ? G : 8);
-    d.splits = (G + d.heads_per_item - 1) / d.heads_per_item;
+    d.split = G > d.heads_per_item ? 1 : 0;
     const int upb = args.block_size / 16;
     d.upb_shift = (upb & (upb - 1)) ? -1 : __builtin_ctz(upb);
     if (args.hd == 64) wide ? launch_decode<64, 2>(d, ws.sms, s, pdl) : launch_decode<64, 1>(d, ws.sms, s, pdl);

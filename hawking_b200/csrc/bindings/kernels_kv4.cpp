@@ -1,7 +1,10 @@
-// torch bindings of the 4-bit paged KV cache kernels (kv4_cache.cu, kv4_attention.cu).
+// torch bindings of the 4-bit paged KV cache kernels (kv4_cache.cu, kv4_decode.cu,
+// kv4_prefill.cu).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+
+#include <cmath>
 
 #include "../kernels/kernels_api.h"
 #include "../kernels/kv4.h"
@@ -205,6 +208,7 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
   TORCH_CHECK((int64_t)a.max_blocks * sh.block_size < (int64_t(1) << 31) - 65536, "kv4 attention: contexts must fit int32");
   a.row_seq = ints(row_seq, a.R, dev, "row_seq");
   a.row_ctx = ints(row_ctx, a.R, dev, "row_ctx");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "kv4 attention: scale must be positive");
   a.scale = (float)scale;
   const auto rows = [&](const optional<Tensor>& t, at::ScalarType ty, int64_t& stride, const char* name) -> void* {
     if (!t.has_value()) return nullptr;
@@ -230,7 +234,7 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
   const hk::Kv4Workspace ws{part.data_ptr<float>(), ints_out(counters, hk::kKv4Counters, dev, "counters"), (int)sms};
   const c10::cuda::CUDAGuard g(dev);
   const cudaStream_t s = at::cuda::getCurrentCUDAStream().stream();
-  if (prefill) hk::kv4_attention_prefill_launch(a, s, pdl);
+  if (prefill) hk::kv4_attention_prefill_launch(a, ws, s, pdl);
   else hk::kv4_attention_decode_launch(a, ws, s, pdl);
 }
 

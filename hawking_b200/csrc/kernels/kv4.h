@@ -1,4 +1,4 @@
-// Host interface of the 4-bit paged KV cache kernels (kv4_cache.cu, kv4_attention.cu).
+// Host interface of the 4-bit paged KV cache kernels (kv4_cache.cu, kv4_decode.cu, kv4_prefill.cu).
 //
 // Cache: [blocks][kv heads][block_size / 16] units; a unit holds 16 tokens of one head in
 // 18 * head_dim bytes (kv4.cuh describes its inside). head_dim is 64, 128 or 256.
@@ -76,12 +76,13 @@ struct Kv4Workspace {
 constexpr int kKv4Counters = 2048;  // decode: three per CTA
 // decode: one CTA per SM, with two partials of its own and one of each of its 15 warps (11 where a partial is
 // larger), of at most 16 heads x (128 + 4) or 8 x (256 + 4) floats
-constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * (2 * 2112 + 11 * 2112); }
+// prefill with split keys: at most one part of 256 rows x (128 + 4) per SM
+constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * 256 * 132; }
 
 void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl);
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl);
 void kv4_gather_launch(const Kv4GatherArgs& a, cudaStream_t s, bool pdl);
 void kv4_attention_decode_launch(const Kv4AttnArgs& a, const Kv4Workspace& ws, cudaStream_t s, bool pdl);
-void kv4_attention_prefill_launch(const Kv4AttnArgs& a, cudaStream_t s, bool pdl);
+void kv4_attention_prefill_launch(const Kv4AttnArgs& a, const Kv4Workspace& ws, cudaStream_t s, bool pdl);
 
 }  // namespace hk

@@ -37,12 +37,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 256;     // (row, head) pairs per CTA
 constexpr int kKeys = 128;     // tokens per tile
 constexpr int kThreads = 512;
+// Registers a thread: at launch, then by role (softmax two warpgroups, unpack and matrix instructions one
+// each). An increase waits for registers that the other roles gave up, so the shares must fit the launch's total.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsUnpack = 112, kRegsIssue = 64;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsUnpack + 128 * kRegsIssue <= kThreads * kRegsLaunch &&
+                  kRegsUnpack <= kRegsLaunch && kRegsIssue <= kRegsLaunch && kRegsSoftmax >= kRegsLaunch,
+              "setmaxnreg shares exceed the block's registers");
 constexpr float kHead = 8.f;   // log2 of how far a score may exceed the reference
 constexpr int kMaxRuns = kRows + 1;
 
 struct PrefillArgs {
   Kv4AttnArgs a;
   int splits;        // parts of the keys (grid.z)
+  int upb_shift;     // log2 of the units per block, or -1
   float* part;       // [grid.x * grid.y * splits][256][HD + 4]
   int* counters;     // [grid.x * grid.y], zero between launches
 };
@@ -62,6 +69,11 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
@@ -106,20 +118,44 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t (&r)[32]) {
       : HK_R4(r, 0), HK_R4(r, 4), HK_R4(r, 8), HK_R4(r, 12), HK_R4(r, 16), HK_R4(r, 20), HK_R4(r, 24), HK_R4(r, 28)
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_x16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::HK_V4(r, 0),
-      HK_V4(r, 4), HK_V4(r, 8), HK_V4(r, 12), HK_V4(r, 16), HK_V4(r, 20), HK_V4(r, 24), HK_V4(r, 28), "r"(addr)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : HK_R4(r, 0), HK_R4(r, 4), HK_R4(r, 8), HK_R4(r, 12)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::HK_V4(r, 0),
+      HK_V4(r, 4), HK_V4(r, 8), HK_V4(r, 12), "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The matrix instructions are issued by one elected lane of a converged warp (their operands then stay in
+// uniform registers).
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, float16 operands
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
       : "memory");
 }
@@ -134,6 +170,9 @@ __device__ __forceinline__ void regs_up() {
 template <int N>
 __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ uint4 ldg16(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
@@ -226,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
   if (z < Z) {
     if (wg < 2) {
       // ================================ softmax ================================
-      regs_up<168>();
+      regs_up<kRegsSoftmax>();
       const int t = wg, i = tid & 127, m = m0 + t * 128 + i;
       const int my_row = m < m_end ? m / G - row0 : -1;  // row of the CTA
       const int head = kvh * G + (m < m_end ? m % G : 0);
@@ -242,12 +281,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         if (t1 > t0) {
           // this thread's query row: float16 after an exact scaling, into the swizzled tile
           const uint16_t* src = a.q + (int64_t)(row0 + max(my_row, 0)) * a.q_stride + (int64_t)head * HD;
+          uint4 qr[HD / 8];
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) {
+            qr[c] = make_uint4(0u, 0u, 0u, 0u);
+            if (mine) qr[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+          }
           __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < HD / 8; ++c) {
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (mine) x = *reinterpret_cast<const uint4*>(src + 8 * c);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            const uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
           }
@@ -258,9 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
           mult = (norm ? __uint_as_float((uint32_t)ex << 23) : 1.f) * (a.scale * kLog2e);
 #pragma unroll
           for (int c = 0; c < HD / 8; ++c) {
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (mine) x = *reinterpret_cast<const uint4*>(src + 8 * c);
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]),
@@ -277,13 +318,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             s_phase ^= 1;
             tc_fence_after();
             const int left = ctx - j * kKeys;  // tokens of the tile that the row sees
+            // 64 scores, those that the row does not see at -infinity, and the largest of them
             uint32_t s[2][32];
-            // 64 scores, those that the row does not see at -infinity
+            const bool edge = __any_sync(0xffffffffu, left < kKeys);
             const auto fetch = [&](int half) {
               tmem_ld_x32(s_at + 64 * half, s[0]);
               tmem_ld_x32(s_at + 64 * half + 32, s[1]);
               tmem_wait_ld();
-              if (left < kKeys) {
+              if (edge) {
 #pragma unroll
                 for (int c = 0; c < 64; ++c) {
                   const int tok = (c & 32) + ((c >> 2) & 1) * 16 + ((c >> 1) & 1) * 8 + ((c >> 3) & 3) * 2 + (c & 1);
@@ -291,16 +333,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
               }
             };
-            float top = -INFINITY;
+            const auto largest = [&](float top) {
+              float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              fetch(half);
-              float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-              for (int c = 0; c < 64; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(s[c >> 5][c & 31]));
-              top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
-            }
-            const float mx = top * mult;
+              for (int c = 0; c < 64; c += 2)
+                t4[(c >> 1) & 3] = max3(t4[(c >> 1) & 3], __uint_as_float(s[c >> 5][c & 31]), __uint_as_float(s[c >> 5][(c & 31) + 1]));
+              return fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]);
+            };
+            fetch(1);
+            const float top = largest(-INFINITY);
+            fetch(0);
+            const float mx = largest(top) * mult;
             const bool move = mx > ref + kHead;
             if (__any_sync(0xffffffffu, move)) {
               const float corr = move ? (ref > -INFINITY ? ex2(ref - mx) : 0.f) : 1.f;
@@ -308,13 +351,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
               l *= corr;
               if (j > t0) {  // the products before this tile's scores are complete: rescale their sum
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld_x32(o_at + c, o);
+                for (int c = 0; c < HD; c += 16) {
+                  uint32_t o[16];
+                  tmem_ld_x16(o_at + c, o);
                   tmem_wait_ld();
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
-                  tmem_st_x32(o_at + c, o);
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                  tmem_st_x16(o_at + c, o);
                 }
               }
             }
@@ -322,21 +365,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const uint64_t mult2 = pack2(mult, mult), base2 = pack2(base, base);
             uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              fetch(c);
-              uint32_t p[32];
+            for (int half = 0; half < 2; ++half) {
+              if (half == 1) fetch(1);  // (the first half's weights lie over its own scores)
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                float lo, hi;
-                unpack2(fma2(pack2(__uint_as_float(s[k >> 4][(2 * k) & 31]), __uint_as_float(s[k >> 4][(2 * k + 1) & 31])),
-                             mult2, base2),
-                        lo, hi);
-                lo = ex2(lo);
-                hi = ex2(hi);
-                sum2[k & 1] = add2(sum2[k & 1], pack2(lo, hi));
-                p[k] = pack_f16(lo, hi);
+              for (int q = 0; q < 2; ++q) {
+                uint32_t p[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  float lo, hi;
+                  unpack2(fma2(pack2(__uint_as_float(s[q][2 * k]), __uint_as_float(s[q][2 * k + 1])), mult2, base2), lo, hi);
+                  lo = ex2(lo);
+                  hi = ex2(hi);
+                  sum2[k & 1] = add2(sum2[k & 1], pack2(lo, hi));
+                  p[k] = pack_f16(lo, hi);
+                }
+                tmem_st_x16(s_at + 32 * half + 16 * q, p);
               }
-              tmem_st_x32(s_at + 32 * c, p);
             }
             float s0, s1;
             unpack2(add2(sum2[0], sum2[1]), s0, s1);
@@ -408,55 +452,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
       }
     } else if (wg == 2) {
       // ================================ unpack ================================
-      regs_down<112>();
-      const int w = warp - 8;                       // tokens 32 w .. of the tile
-      const int b = (lane >> 2) & 1, kt = lane & 3, kx = lane >> 3;  // keys: unit 2 w + b, word column, token 4 i + kx
-      const int vt = lane & 3;                      // values: tokens 2 vt, + 1 of each 8
+      regs_down<kRegsUnpack>();
+      const int w = warp & 3;  // tokens 32 w .. of the tile: units 2 w, 2 w + 1
       const int upb = a.block_size / 16;
       int n_done = 0;
-      for (int run = 0; run < n_runs && ok; ++run) {
-        int t0, t1;
-        tiles_of(run, t0, t1);
-        const int kv_len = run_kv[run], units = (kv_len + 15) >> 4;
-        if (t1 <= t0) continue;
-        const int* table = a.block_tables + (int64_t)seq_s[run_at[run]] * a.max_blocks;
-        // unit u of the sequence, or null past its end; a block outside the cache reads as zeros
-        const auto unit_at = [&](int u) -> const uint8_t* {
-          if (u >= units) return nullptr;
-          const int blk = table[u / upb];
-          if (blk < 0 || blk >= a.cache_blocks) {
-            set_error(a.status, HK_ERR_BAD_ARG);
-            return nullptr;
-          }
-          return a.cache + (((int64_t)blk * a.nkv + kvh) * upb + u % upb) * U::kBytes;
-        };
-        uint4 kr[4];         // keys: 16 bytes (HD 64: 8) of tokens 4 i + kx
-        uint2 kp[4];         // their pairs
-        uint4 vr[2][GR];     // values: 16 bytes of units 2 w, 2 w + 1
-        uint4 vp[2][2];      // pairs of tokens 8 h + 2 vt, + 1
-        const auto load = [&](int j) {
-          const uint8_t* u0 = unit_at(8 * j + 2 * w);
-          const uint8_t* u1 = unit_at(8 * j + 2 * w + 1);
-          const uint8_t* ku = b ? u1 : u0;
+      const int* table = nullptr;
+      int units = 0;
+      // block of unit u (-1 past the sequence's end), and the unit's bytes; a block outside the cache reads as zeros
+      const auto block_of = [&](int u) {
+        return u < units ? table[g_.upb_shift >= 0 ? u >> g_.upb_shift : u / upb] : -1;
+      };
+      const auto unit_at = [&](int u, int blk) -> const uint8_t* {
+        if (blk < 0 || blk >= a.cache_blocks) {
+          if (u < units) set_error(a.status, HK_ERR_BAD_ARG);
+          return nullptr;
+        }
+        const int in = g_.upb_shift >= 0 ? u & (upb - 1) : u % upb;
+        return a.cache + (((int64_t)blk * a.nkv + kvh) * upb + in) * U::kBytes;
+      };
+      // keys: a thread has 16 bytes (HD 64: 8) of tokens 4 i + kx of unit 2 w + b
+      const int b = (lane >> 2) & 1, kt = lane & 3, kx = lane >> 3;
+      // values: 16 bytes of both units, tokens 8 h + 2 vt, + 1 of dims 4 vg .. of each 32
+      const int vt = lane & 3, vg = lane >> 2;
+      {
+        for (int run = 0; run < n_runs && ok; ++run) {
+          int t0, t1;
+          tiles_of(run, t0, t1);
+          if (t1 <= t0) continue;
+          const int kv_len = run_kv[run];
+          units = (kv_len + 15) >> 4;
+          table = a.block_tables + (int64_t)seq_s[run_at[run]] * a.max_blocks;
+          uint4 kr[4];
+          uint2 kp[4];
+          const auto load_k = [&](const uint8_t* ku) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            kr[i] = make_uint4(0u, 0u, 0u, 0u);
-            kp[i] = make_uint2(0u, 0u);
-            if (ku) {
-              const int tok = 4 * i + kx;
-              if (HD == 64) {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(ku + tok * U::kRow + kt * 8));
-                kr[i].x = x.x, kr[i].y = x.y;
-                kp[i].x = __ldg(reinterpret_cast<const uint32_t*>(ku + U::pair(false, tok, 0)));
-              } else {
-                kr[i] = ldg16(ku + tok * U::kRow + kt * 16);
-                kp[i] = __ldg(reinterpret_cast<const uint2*>(ku + U::pair(false, tok, 0)));
+            for (int i = 0; i < 4; ++i) {
+              kr[i] = make_uint4(0u, 0u, 0u, 0u);
+              kp[i] = make_uint2(0u, 0u);
+              if (ku) {
+                const int tok = 4 * i + kx;
+                if (HD == 64) {
+                  const uint2 x = __ldg(reinterpret_cast<const uint2*>(ku + tok * U::kRow + kt * 8));
+                  kr[i].x = x.x, kr[i].y = x.y;
+                  kp[i].x = __ldg(reinterpret_cast<const uint32_t*>(ku + U::pair(false, tok, 0)));
+                } else {
+                  kr[i] = ldg16(ku + tok * U::kRow + kt * 16);
+                  kp[i] = __ldg(reinterpret_cast<const uint2*>(ku + U::pair(false, tok, 0)));
+                }
               }
             }
-          }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint8_t* vu = x ? u1 : u0;
+          };
+          uint4 vr[2][GR];  // values of units 2 w, 2 w + 1
+          uint4 vp[2][2];   // pairs of tokens 8 h + 2 vt, + 1
+          const auto load_v = [&](int x, const uint8_t* vu) {
 #pragma unroll
             for (int g = 0; g < GR; ++g) {
               vr[x][g] = make_uint4(0u, 0u, 0u, 0u);
@@ -475,80 +523,114 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
               }
             }
-          }
-        };
-        load(t0);
-        for (int j = t0; j < t1; ++j, ++n_done) {
-          const int st = n_done & 1, free_phase = ((n_done >> 1) & 1) ^ 1;
-          if (!(ok = mbar_wait(&k_empty[st], free_phase, a.status))) break;
-          uint8_t* ks = smem + Sh::kOffK + st * Sh::kKStage;
+          };
+          const auto load = [&](int u, int blk0, int blk1) {
+            const uint8_t *u0 = unit_at(u, blk0), *u1 = unit_at(u + 1, blk1);
+            load_k(b ? u1 : u0);
+            load_v(0, u0);
+            load_v(1, u1);
+          };
+          int u = 8 * t0 + 2 * w;
+          load(u, block_of(u), block_of(u + 1));
+          int blk0 = block_of(u + 8), blk1 = block_of(u + 9);  // of the tile after the loaded one
+          for (int j = t0; j < t1; ++j, ++n_done) {
+            const int st = n_done & 1;
+            if (!(ok = mbar_wait(&k_empty[st], ((n_done >> 1) & 1) ^ 1, a.status))) break;
+            const uint32_t ks = smem_k + st * Sh::kKStage + (32 * w + (kx >> 1) * 8 + b * 4 + (kx & 1)) * 128;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 32 * w + (2 * (i & 1) + (kx >> 1)) * 8 + b * 4 + (i >> 1) * 2 + (kx & 1);
-            const uint32_t x[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
+            for (int i = 0; i < 4; ++i) {
+              // row 32 w + 8 (2 (i & 1) + (kx >> 1)) + 4 b + 2 (i >> 1) + (kx & 1) of the tile
+              const int r = (2 * (i & 1)) * 8 + (i >> 1) * 2;
+              const uint32_t x[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
 #pragma unroll
-            for (int k = 0; k < HD / 32; ++k) {
-              const __half2 p = as_h2(k < 2 ? kp[i].x : kp[i].y);
-              const __half2 s = __low2half2(p), c = __high2half2(p);
-              *reinterpret_cast<uint4*>(ks + (k >> 1) * Sh::kAtom + sw128_offset(r, 4 * (k & 1) + kt)) =
-                  make_uint4(value_even(x[k], s, c), value_odd(x[k], s, c), value_even(x[k] >> 8, s, c),
-                             value_odd(x[k] >> 8, s, c));
+              for (int k = 0; k < HD / 32; ++k) {
+                const __half2 p = as_h2(k < 2 ? kp[i].x : kp[i].y);
+                const __half2 s = __low2half2(p), c = __high2half2(p);
+                const int chunk = (4 * (k & 1) + kt) ^ (4 * b + 2 * (i >> 1) + (kx & 1));
+                sts16(ks + (k >> 1) * Sh::kAtom + r * 128 + chunk * 16, value_even(x[k], s, c), value_odd(x[k], s, c),
+                      value_even(x[k] >> 8, s, c), value_odd(x[k] >> 8, s, c));
+              }
             }
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&k_full[st]);
-          if (!(ok = mbar_wait(&v_empty[st], free_phase, a.status))) break;
-          uint8_t* vs = smem + Sh::kOffV + st * Sh::kVStage + (w >> 1) * HD * 128;
-#pragma unroll
-          for (int g = 0; g < GR; ++g) {
-            __half2 s[2][2], c[2][2];
+            fence_proxy_async_smem();
+            mbar_arrive(&k_full[st]);
+            // scales and centres of the token pairs [unit][half][group]
+            uint32_t s2[2][2][GR], c2[2][2][GR];
+            __half2 odd = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+            const __half2 zero = odd;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t p0 = g ? vp[x][h].y : vp[x][h].x, p1 = g ? vp[x][h].w : vp[x][h].z;
-                uint32_t s2 = __byte_perm(p0, p1, 0x5410), c2 = __byte_perm(p0, p1, 0x7632);
-                const int tok = j * kKeys + 32 * w + 16 * x + 8 * h + 2 * vt;
-                // tokens past the end hold stale bytes; NaN is noted instead
-                const bool odd0 = (~s2 & 0x7c00u) == 0 || (~c2 & 0x7c00u) == 0;
-                const bool odd1 = (~s2 & 0x7c000000u) == 0 || (~c2 & 0x7c000000u) == 0;
-                const bool end0 = tok >= kv_len, end1 = tok + 1 >= kv_len;
-                if (odd0 && !end0) atomicMin(&nan_at[run][g], tok);
-                if (odd1 && !end1) atomicMin(&nan_at[run][g], tok + 1);
-                const uint32_t keep = (odd0 || end0 ? 0u : 0xffffu) | (odd1 || end1 ? 0u : 0xffff0000u);
-                s[x][h] = as_h2(s2 & keep);
-                c[x][h] = as_h2(c2 & keep);
-              }
+              for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int il = 0; il < 2; ++il) {
-              uint32_t x[2][2];
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                x[y][0] = il ? vr[y][g].z : vr[y][g].x;
-                x[y][1] = il ? vr[y][g].w : vr[y][g].y;
-              }
-#pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                uint32_t o[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  const uint32_t v = p < 2 ? x[y >> 1][y & 1] : x[y >> 1][y & 1] >> 8;
-                  o[y] = p & 1 ? value_odd(v, s[y >> 1][y & 1], c[y >> 1][y & 1]) : value_even(v, s[y >> 1][y & 1], c[y >> 1][y & 1]);
+                for (int g = 0; g < GR; ++g) {
+                  const uint32_t p0 = g ? vp[x][h].y : vp[x][h].x, p1 = g ? vp[x][h].w : vp[x][h].z;
+                  s2[x][h][g] = __byte_perm(p0, p1, 0x5410);
+                  c2[x][h][g] = __byte_perm(p0, p1, 0x7632);
+                  odd = __hfma2(as_h2(s2[x][h][g]), zero, __hfma2(as_h2(c2[x][h][g]), zero, odd));
                 }
-                const int d = 64 * g + 32 * il + 4 * (lane >> 2) + p;
-                *reinterpret_cast<uint4*>(vs + sw128_offset(d, 4 * (w & 1) + vt)) = make_uint4(o[0], o[1], o[2], o[3]);
+            // the sequence's last tokens hold stale bytes past its end; NaN is noted: both become zeros
+            const bool end = (j + 1) * kKeys > kv_len;
+            if (end || (as_u32(odd) & 0x7fff7fffu)) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int g = 0; g < GR; ++g) {
+                    const int tok = j * kKeys + 32 * w + 16 * x + 8 * h + 2 * vt;
+                    const uint32_t sv = s2[x][h][g], cv = c2[x][h][g];
+                    const bool odd0 = (~sv & 0x7c00u) == 0 || (~cv & 0x7c00u) == 0;
+                    const bool odd1 = (~sv & 0x7c000000u) == 0 || (~cv & 0x7c000000u) == 0;
+                    const bool end0 = tok >= kv_len, end1 = tok + 1 >= kv_len;
+                    if (odd0 && !end0) atomicMin(&nan_at[run][g], tok);
+                    if (odd1 && !end1) atomicMin(&nan_at[run][g], tok + 1);
+                    const uint32_t keep = (odd0 || end0 ? 0u : 0xffffu) | (odd1 || end1 ? 0u : 0xffff0000u);
+                    s2[x][h][g] = sv & keep;
+                    c2[x][h][g] = cv & keep;
+                  }
+            }
+            if (!(ok = mbar_wait(&v_empty[st], ((n_done >> 1) & 1) ^ 1, a.status))) break;
+            const uint32_t vs = smem_v + st * Sh::kVStage + (w >> 1) * HD * 128 + 4 * vg * 128;
+#pragma unroll
+            for (int g = 0; g < GR; ++g)
+#pragma unroll
+              for (int il = 0; il < 2; ++il) {
+                uint32_t x[2][2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  x[y][0] = il ? vr[y][g].z : vr[y][g].x;
+                  x[y][1] = il ? vr[y][g].w : vr[y][g].y;
+                }
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                  uint32_t o[4];
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) {
+                    const int xx = y >> 1, h = y & 1;
+                    const uint32_t v = p < 2 ? x[xx][h] : x[xx][h] >> 8;
+                    o[y] = p & 1 ? value_odd(v, as_h2(s2[xx][h][g]), as_h2(c2[xx][h][g]))
+                                 : value_even(v, as_h2(s2[xx][h][g]), as_h2(c2[xx][h][g]));
+                  }
+                  // row 64 g + 32 il + 4 vg + p
+                  const int chunk = (4 * (w & 1) + vt) ^ (4 * (vg & 1) + p);
+                  sts16(vs + (64 * g + 32 * il + p) * 128 + chunk * 16, o[0], o[1], o[2], o[3]);
+                }
               }
+            fence_proxy_async_smem();
+            mbar_arrive(&v_full[st]);
+            if (j + 1 < t1) {
+              u += 8;
+              load(u, blk0, blk1);
+              blk0 = block_of(u + 8);
+              blk1 = block_of(u + 9);
             }
           }
-          fence_proxy_async_smem();
-          mbar_arrive(&v_full[st]);
-          if (j + 1 < t1) load(j + 1);
         }
       }
     } else {
       // ================================ matrix instructions ================================
-      regs_down<64>();
-      if (warp == 12 && lane == 0) {
+      regs_down<kRegsIssue>();
+      if (warp == 12) {
         constexpr uint32_t id_s = idesc_f16_f32(128, kKeys), id_o = idesc_f16_f32(128, HD);
         int n_k = 0, n_v = 0, p_phase = 0, q_phase = 0;
         // (descriptor addresses count 16 bytes)
@@ -560,9 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const uint32_t off = at * (Sh::kAtom >> 4) + k * 2;
-              umma_f16(tmem + t * 128, q0 + off, k0 + off, id_s, (at | k) > 0);
+              umma_f16_ss(tmem + t * 128, q0 + off, k0 + off, id_s, (at | k) > 0);
             }
-          umma_commit(&s_ready[t]);
+          commit_elected(&s_ready[t]);
         };
         const auto output = [&](int t, int st, bool more) {
           const uint64_t v0 = dv + st * (Sh::kVStage >> 4);
@@ -583,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
           tc_fence_after();
           scores(0, n_k & 1);
           scores(1, n_k & 1);
-          umma_commit(&k_empty[n_k & 1]);
+          commit_elected(&k_empty[n_k & 1]);
           ++n_k;
           for (int j = t0; j < t1 && ok; ++j, ++n_v) {
             const int vst = n_v & 1, kst = n_k & 1;
@@ -596,10 +678,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
               if (!ok) break;
               tc_fence_after();
               output(t, vst, j > t0);
-              if (t == 1) umma_commit(&v_empty[vst]);
+              if (t == 1) commit_elected(&v_empty[vst]);
               if (more) scores(t, kst);
-              else umma_commit(&o_done[t]);
-              if (more && t == 1) umma_commit(&k_empty[kst]);
+              else commit_elected(&o_done[t]);
+              if (more && t == 1) commit_elected(&k_empty[kst]);
             }
             if (more) ++n_k;
             p_phase ^= 1;
@@ -679,6 +761,10 @@ void launch_prefill(const PrefillArgs& p, dim3 grid, cudaStream_t s, bool pdl) {
   if (!configured) {
     HK_CUDA_CHECK(cudaFuncSetAttribute(kv4_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        PrefillShape<HD>::kSmem));
+    cudaFuncAttributes at;
+    HK_CUDA_CHECK(cudaFuncGetAttributes(&at, kv4_prefill_kernel<HD>));
+    // (the register shares count on it: a smaller allocation would leave the increases waiting)
+    if (at.numRegs != kRegsLaunch) throw std::runtime_error("kv4 attention prefill: built with another register count");
     configured = true;
   }
   launch(kv4_prefill_kernel<HD>, grid, dim3(kThreads), PrefillShape<HD>::kSmem, s, pdl, p);
@@ -695,6 +781,8 @@ void kv4_attention_prefill_launch(const Kv4AttnArgs& args, const Kv4Workspace& w
   p.part = ws.part;
   p.counters = ws.counters;
   // with fewer CTAs than SMs the keys are split over the rest
+  const int upb = args.block_size / 16;
+  p.upb_shift = (upb & (upb - 1)) ? -1 : __builtin_ctz(upb);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(32, ws.sms / (tiles * args.nkv)));
   const dim3 grid(args.nkv, (unsigned)tiles, p.splits);
   if (args.hd == 64) launch_prefill<64>(p, grid, s, pdl);

@@ -42,6 +42,20 @@ struct Unit {
   }
 };
 
+// Codes less 8, exact, as float16 pairs of the even (0x000f000f) and odd (0x00f000f0) nibbles of w: 1024 + m
+// and 1024 + 16 m are the bit patterns themselves.
+__device__ __forceinline__ uint32_t centre_even(uint32_t w) {
+  const uint32_t x = (w & 0x000f000fu) | 0x64006400u, k = 0xe408e408u;  // -1032
+  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t centre_odd(uint32_t w) {
+  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u, s = 0x2c002c00u, k = 0xd480d480u;  // 1 / 16, -72
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&s),
+                            *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // Largest magnitude a group holds: larger finite values are clamped to it, so that the centre and
 // the ends c - 8 s, c + 7 s of every group stay finite in float16.
 constexpr float kMaxValue = 65024.f;

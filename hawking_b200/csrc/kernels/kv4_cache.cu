@@ -114,10 +114,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
 }
 
 // ---- RoPE + quantise + append ----------------------------------------------------------------------
-// One warp per head row (two heads per warp at HD 64): every lane holds 4 consecutive dims of each
-// 128 (or 64), so that 16 lanes hold the 64 dims of a quantisation group. Products and sums of the
-// rotation are rounded one by one and the codes use exact divisions, so the bytes written do not
-// depend on how the compiler contracts them.
+// A warp takes HB heads of one row (HB pairs of heads at HD 64), so that the position's rotation is read once
+// for them and all their loads are in flight together: at 2048 rows of 48 heads HB = 4 against 1 measured
+// FIG_HB; a few rows keep one head per warp (the launch needs warps more than the warps need work).
+// Every lane holds 4 consecutive dims of each 128 (or 64), 16 lanes the 64 dims of a quantisation group.
+// Sums, products and divisions are rounded one by one, the norm's sum of squares in a fixed order,
+// so the bytes written do not depend on how the compiler contracts them.
 struct Vec4 {
   float v[4];
 };
@@ -126,192 +128,312 @@ __device__ __forceinline__ Vec4 ld4(const float* p) {
   return {{f.x, f.y, f.z, f.w}};
 }
 
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendArgs a) {
+template <int HD, int HB>
+__global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
   constexpr int LG = HD < 128 ? HD / 4 : 32;  // lanes of one head
-  constexpr int HPW = 32 / LG;                // heads per warp
+  constexpr int HPW = 32 / LG;                // heads side by side in a warp
   constexpr int NV = HD / (4 * LG);           // vectors of 4 dims per lane
   using U = Unit<HD>;
   pdl_wait();
   const int lane = threadIdx.x & 31, sl = lane % LG;
-  const int heads = a.nh + 2 * a.nkv, per_row = (heads + HPW - 1) / HPW;
-  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (unit >= (int64_t)a.R * per_row) return;
-  const int r = (int)(unit / per_row);
-  const int h = (int)(unit % per_row) * HPW + lane / LG;
-  const bool live = h < heads;
-  const int hc = live ? h : heads - 1;  // lanes without a head compute on the last one and store nothing
+  const int heads = a.nh + 2 * a.nkv, per_row = (heads + HPW * HB - 1) / (HPW * HB);
+  const int r = blockIdx.x, unit = blockIdx.y * 4 + (threadIdx.x >> 5);
+  if (unit >= per_row) return;
+  const int h0 = unit * (HPW * HB) + lane / LG;
+  const float* row = a.qkv + (int64_t)r * a.qkv_stride;
+  Vec4 x[HB][NV];
+#pragma unroll
+  for (int b = 0; b < HB; ++b)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)  // (lanes without a head compute on the last one and store nothing)
+      x[b][j] = ld4(row + (int64_t)min(h0 + b * HPW, heads - 1) * HD + 128 * j + 4 * sl);
   const int pos = a.positions[r];
   if (pos < 0 || pos >= a.rope_rows) return;  // the whole warp
-  const int kind = hc < a.nh ? 0 : (hc < a.nh + a.nkv ? 1 : 2);  // q, k, v
-  const float* src = a.qkv + (int64_t)r * a.qkv_stride + (int64_t)hc * HD;
-  const float* bias = a.bias ? a.bias + (int64_t)hc * HD : nullptr;
-  const float* nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
-  Vec4 x[NV];
+  int64_t slot = -1;
+  if (__any_sync(0xffffffffu, h0 + (HB - 1) * HPW >= a.nh)) {  // keys or values among the heads
+    if (a.slots) {
+      slot = a.slots[r];
+    } else {
+      const int seq = a.row_seq[r], col = pos / a.block_size;
+      if (seq >= 0 && seq < a.table_rows && col < a.max_blocks)
+        slot = (int64_t)a.block_tables[(int64_t)seq * a.max_blocks + col] * a.block_size + pos % a.block_size;
+    }
+  }
+  const bool keep = slot >= 0 && slot < a.cache_blocks * a.block_size;
+  int blk = 0, off = 0;
+  if (keep) {
+    blk = (int)slot / a.block_size;  // (the pool holds less than 2^31 tokens)
+    off = (int)slot - blk * a.block_size;
+  }
+  const int tok = off & 15;
+  // this lane's rotations: adjacent pairs, or halves (cos, sin of dims d and, with the sign, their partners)
+  const int half = a.rot_dim / 2;
+  const float* rope = a.rope + (int64_t)pos * a.rot_dim;
+  float cs[NV][4], sn[NV][4];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    x[j] = ld4(src + 128 * j + 4 * sl);
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 128 * j + 4 * sl + e;
+      cs[j][e] = 1.f;
+      sn[j][e] = 0.f;
+      if (d < a.rot_dim) {
+        const int i = a.rope_style == 0 ? d >> 1 : (d < half ? d : d - half);
+        const float2 t = *reinterpret_cast<const float2*>(rope + 2 * i);
+        cs[j][e] = t.x;
+        sn[j][e] = t.y;
+      }
+    }
+#pragma unroll
+  for (int b = 0; b < HB; ++b) {
+    const int h = h0 + b * HPW;
+    const bool live = h < heads;
+    const int hc = min(h, heads - 1);
+    const int kind = hc < a.nh ? 0 : (hc < a.nh + a.nkv ? 1 : 2);  // q, k, v
+    const float* src = row + (int64_t)hc * HD;
+    const float* bias = a.bias ? a.bias + (int64_t)hc * HD : nullptr;
+    const float* nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
+    Vec4(&v)[NV] = x[b];
     if (bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j].v[e] += bias[128 * j + 4 * sl + e];
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j].v[e] = __fadd_rn(v[j].v[e], bias[128 * j + 4 * sl + e]);
     }
-  }
-  float inv = 1.f;
-  {
-    float ss = 0.f;
+    float inv = 1.f;
+    if (a.q_norm || a.k_norm) {  // (the same for the warp)
+      float ss[4];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+      for (int e = 0; e < 4; ++e) {
+        ss[e] = __fmul_rn(v[0].v[e], v[0].v[e]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ss += x[j].v[e] * x[j].v[e];
-#pragma unroll
-    for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (nw) inv = rsqrtf(ss / HD + a.eps);
-  }
-  if (nw) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[j].v[e] = __fmul_rn(__fmul_rn(x[j].v[e], inv), nw[128 * j + 4 * sl + e]);
-  }
-  if (kind < 2) {
-    const int half = a.rot_dim / 2;
-    const float* rope = a.rope + (int64_t)pos * a.rot_dim;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int d0 = 128 * j + 4 * sl;
-      if (a.rope_style == 0) {  // pairs (d, d + 1)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          if (d0 + e < a.rot_dim) {
-            const float2 cs = *reinterpret_cast<const float2*>(rope + d0 + e);
-            const float p = x[j].v[e], q = x[j].v[e + 1];
-            x[j].v[e] = __fsub_rn(__fmul_rn(p, cs.x), __fmul_rn(q, cs.y));
-            x[j].v[e + 1] = __fadd_rn(__fmul_rn(p, cs.y), __fmul_rn(q, cs.x));
-          }
-        }
-      } else {  // pairs (d, d + half): the partner is read again (an L1 hit), normalised alike
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = d0 + e;
-          if (d < a.rot_dim) {
-            const bool first = d < half;
-            const int o = first ? d + half : d - half;
-            float y = src[o] + (bias ? bias[o] : 0.f);
-            if (nw) y = __fmul_rn(__fmul_rn(y, inv), nw[o]);
-            const float2 cs = *reinterpret_cast<const float2*>(rope + 2 * (first ? d : o));
-            x[j].v[e] = first ? __fsub_rn(__fmul_rn(x[j].v[e], cs.x), __fmul_rn(y, cs.y))
-                              : __fadd_rn(__fmul_rn(y, cs.y), __fmul_rn(x[j].v[e], cs.x));
-          }
-        }
+        for (int j = 1; j < NV; ++j) ss[e] = __fadd_rn(ss[e], __fmul_rn(v[j].v[e], v[j].v[e]));
       }
-    }
-  }
-  if (kind == 0 && live) {
-    uint16_t* dst = a.q_out + (int64_t)r * a.q_stride + (int64_t)h * HD;
+      // 64 dims in halves all the way down, more dims four in a row and then in halves
+      float sum;
+      if (HD == 64) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(x[j].v[0], x[j].v[1]);
-      const __nv_bfloat162 hi = __floats2bfloat162_rn(x[j].v[2], x[j].v[3]);
-      *reinterpret_cast<uint2*>(dst + 128 * j + 4 * sl) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    }
-  }
-  if (!__any_sync(0xffffffffu, kind != 0)) return;
-  int64_t slot = -1;
-  if (a.slots) {
-    slot = a.slots[r];
-  } else {
-    const int seq = a.row_seq[r], col = pos / a.block_size;
-    if (seq >= 0 && seq < a.table_rows && col < a.max_blocks)
-      slot = (int64_t)a.block_tables[(int64_t)seq * a.max_blocks + col] * a.block_size + pos % a.block_size;
-  }
-  const bool store = live && kind != 0 && slot >= 0 && slot < a.cache_blocks * a.block_size;
-  const int kh = kind == 1 ? hc - a.nh : hc - a.nh - a.nkv;
-  const int64_t blk = store ? slot / a.block_size : 0;
-  const int off = store ? (int)(slot % a.block_size) : 0, tok = off & 15;
-  uint8_t* u = a.cache + ((blk * a.nkv + (store ? kh : 0)) * (a.block_size / 16) + off / 16) * U::kBytes;
+        for (int o = LG / 2; o > 0; o >>= 1)
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    bool odd = false;  // a NaN or an infinity in the group
-    float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float& t = x[j].v[e];
-      odd |= !(fabsf(t) < INFINITY);
-      t = fminf(fmaxf(t, -kv4::kMaxValue), kv4::kMaxValue);
-      lo = fminf(lo, t);
-      hi = fmaxf(hi, t);
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 16) & 0xffffu) != 0;
-    __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
-    const float s = __half2float(sh);
-    __half ch = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, s)));
-    const float c = __half2float(ch);
-    uint32_t code[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float q = s > 0.f ? __fadd_rn(rintf(__fdiv_rn(__fsub_rn(x[j].v[e], c), s)), 8.f) : 8.f;
-      code[e] = odd ? 8u : (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
-    }
-    if (odd) sh = ch = __ushort_as_half(0x7fff);  // such a group reads back as NaN
-    // key words hold 8 dims: two lanes' parts
-    uint32_t w = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20;
-    w <<= (lane & 1) * 8;
-    w |= __shfl_xor_sync(0xffffffffu, w, 1);
-    if (store) {
-      const int d = 128 * j + 4 * sl;
-      if (kind == 1) {
-        if ((lane & 1) == 0) *reinterpret_cast<uint32_t*>(u + U::key_word(tok, d)) = w;
+          for (int e = 0; e < 4; ++e) ss[e] = __fadd_rn(ss[e], __shfl_xor_sync(0xffffffffu, ss[e], o));
+        sum = __fadd_rn(__fadd_rn(ss[0], ss[2]), __fadd_rn(ss[1], ss[3]));
       } else {
-        *reinterpret_cast<uint16_t*>(u + U::value_half(tok, d)) =
-            (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+        sum = __fadd_rn(__fadd_rn(__fadd_rn(ss[0], ss[1]), ss[2]), ss[3]);
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
       }
-      if ((lane & 15) == 0) *reinterpret_cast<__half2*>(u + U::pair(kind == 2, tok, d >> 6)) = __halves2half2(sh, ch);
+      if (nw) {
+        inv = rsqrtf(__fadd_rn(__fmul_rn(sum, 1.f / HD), a.eps));
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j].v[e] = __fmul_rn(__fmul_rn(v[j].v[e], inv), nw[128 * j + 4 * sl + e]);
+      }
+    }
+    if (kind < 2) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int d0 = 128 * j + 4 * sl;
+        if (a.rope_style == 0) {  // pairs (d, d + 1)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            if (d0 + e < a.rot_dim) {
+              const float p = v[j].v[e], q = v[j].v[e + 1];
+              v[j].v[e] = __fsub_rn(__fmul_rn(p, cs[j][e]), __fmul_rn(q, sn[j][e]));
+              v[j].v[e + 1] = __fadd_rn(__fmul_rn(p, sn[j][e]), __fmul_rn(q, cs[j][e]));
+            }
+          }
+        } else {  // pairs (d, d + half): the partner is read again (an L1 hit), normalised alike
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = d0 + e;
+            if (d < a.rot_dim) {
+              const bool first = d < half;
+              const int o = first ? d + half : d - half;
+              float y = src[o];
+              if (bias) y = __fadd_rn(y, bias[o]);
+              if (nw) y = __fmul_rn(__fmul_rn(y, inv), nw[o]);
+              v[j].v[e] = first ? __fsub_rn(__fmul_rn(v[j].v[e], cs[j][e]), __fmul_rn(y, sn[j][e]))
+                                : __fadd_rn(__fmul_rn(y, sn[j][e]), __fmul_rn(v[j].v[e], cs[j][e]));
+            }
+          }
+        }
+      }
+    }
+    if (kind == 0 && live) {
+      uint16_t* dst = a.q_out + (int64_t)r * a.q_stride + (int64_t)h * HD;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[j].v[0], v[j].v[1]);
+        const __nv_bfloat162 hi = __floats2bfloat162_rn(v[j].v[2], v[j].v[3]);
+        *reinterpret_cast<uint2*>(dst + 128 * j + 4 * sl) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+    }
+    if (!__any_sync(0xffffffffu, kind != 0 && live && keep)) continue;
+    const bool store = live && kind != 0 && keep;
+    const int kh = kind == 0 ? 0 : (kind == 1 ? hc - a.nh : hc - a.nh - a.nkv);
+    uint8_t* u = a.cache + (((int64_t)blk * a.nkv + kh) * (a.block_size / 16) + off / 16) * U::kBytes;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      bool odd = false;  // a NaN or an infinity in the group
+      float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float& t = v[j].v[e];
+        odd |= !(fabsf(t) < INFINITY);
+        t = fminf(fmaxf(t, -kv4::kMaxValue), kv4::kMaxValue);
+        lo = fminf(lo, t);
+        hi = fmaxf(hi, t);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 16) & 0xffffu) != 0;
+      __half sh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
+      const float s = __half2float(sh);
+      __half ch = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, s)));
+      const float c = __half2float(ch);
+      uint32_t code[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float q = s > 0.f ? __fadd_rn(rintf(__fdiv_rn(__fsub_rn(v[j].v[e], c), s)), 8.f) : 8.f;
+        code[e] = odd ? 8u : (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
+      }
+      if (odd) sh = ch = __ushort_as_half(0x7fff);  // such a group reads back as NaN
+      // key words hold 8 dims: two lanes' parts
+      uint32_t w = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20;
+      w <<= (lane & 1) * 8;
+      w |= __shfl_xor_sync(0xffffffffu, w, 1);
+      if (store) {
+        const int d = 128 * j + 4 * sl;
+        if (kind == 1) {
+          if ((lane & 1) == 0) *reinterpret_cast<uint32_t*>(u + U::key_word(tok, d)) = w;
+        } else {
+          *reinterpret_cast<uint16_t*>(u + U::value_half(tok, d)) =
+              (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+        }
+        if ((lane & 15) == 0) *reinterpret_cast<__half2*>(u + U::pair(kind == 2, tok, d >> 6)) = __halves2half2(sh, ch);
+      }
     }
   }
   pdl_launch();
 }
 
 // ---- gather ----------------------------------------------------------------------------------------
-// 4 dims of one token's head per thread (K and V): 8-byte stores, coalesced over the dims.
+// A warp takes 16 slots of one head. Where they are the 16 tokens of a unit in order, as a sequence's slots
+// are, it reads the unit whole, in its own order: a lane's 16 bytes of key codes are 4 x 8 dims of a token, its
+// 16 bytes of value codes 2 x 4 dims of four tokens, so loads and stores are whole sectors and a code costs
+// FIG_GATHER. Any other slots go token by token, 4 dims per lane.
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, float2 p) {  // centred codes (float16 pair), (s, c)
+  const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&codes));
+  const __nv_bfloat162 v = __floats2bfloat162_rn(fmaf(p.x, n.x, p.y), fmaf(p.x, n.y, p.y));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(Kv4GatherArgs a) {
   using U = Unit<HD>;
+  constexpr int GR = HD / 64;
   pdl_wait();
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t total = (int64_t)a.N * a.nkv * (HD / 4);
-  if (i >= total) return;
-  const int d = (int)(i % (HD / 4)) * 4;
-  const int64_t th = i / (HD / 4);
-  const int h = (int)(th % a.nkv);
-  const int64_t slot = a.slots[th / a.nkv];
-  float k[4] = {}, v[4] = {};
-  if (slot >= 0 && slot < a.cache_blocks * a.block_size) {
-    const int off = (int)(slot % a.block_size), tok = off & 15;
-    const uint8_t* u =
-        a.cache + (((slot / a.block_size) * a.nkv + h) * (a.block_size / 16) + off / 16) * U::kBytes;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(u + U::key_word(tok, d & ~7)) >> ((d & 4) * 2);
-    const uint32_t vw = *reinterpret_cast<const uint16_t*>(u + U::value_half(tok, d));
-    const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(u + U::pair(false, tok, d >> 6)));
-    const float2 vp = __half22float2(*reinterpret_cast<const __half2*>(u + U::pair(true, tok, d >> 6)));
+  const int lane = threadIdx.x & 31;
+  if (blockIdx.y == 0) a.v = nullptr;  // keys and values by different warps: short lists are a matter of latency
+  else a.k = nullptr;
+  const int64_t task = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t groups = (a.N + 15) / 16;
+  if (task >= groups * a.nkv) return;
+  const int64_t i0 = task / a.nkv * 16;
+  const int h = (int)(task % a.nkv), n = (int)min((int64_t)16, a.N - i0);
+  const int64_t pool = a.cache_blocks * a.block_size;
+  const int mine = lane < n ? a.slots[i0 + lane] : -1;
+  const int first = __shfl_sync(0xffffffffu, mine, 0);
+  const bool run = __all_sync(0xffffffffu, lane >= n || mine == first + lane) && n == 16 && first >= 0 &&
+                   (first & 15) == 0 && first < pool;
+  if (run) {
+    const int blk = first / a.block_size, off = first - blk * a.block_size;
+    const uint8_t* u = a.cache + (((int64_t)blk * a.nkv + h) * (a.block_size / 16) + off / 16) * U::kBytes;
+    const int64_t out = (i0 * a.nkv + h) * HD;
+    const int64_t step = (int64_t)a.nkv * HD;  // to the next token's row
+    if (a.k) {
+      constexpr int W = HD < 128 ? 2 : 4;  // words of a token in a plane
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      k[e] = fmaf(kp.x, (float)((int)(kw >> ((e >> 1) * 4 + (e & 1) * 16) & 15u) - 8), kp.y);
-      v[e] = fmaf(vp.x, (float)((int)(vw >> (4 * e) & 15u) - 8), vp.y);
+      for (int pl = 0; pl < (HD + 127) / 128; ++pl)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int tok = 8 * x + (lane >> 2), t = lane & 3;
+          const uint8_t* src = u + pl * 16 * U::kRow + tok * U::kRow + t * (U::kRow / 4);
+          uint32_t w[4];
+          if (W == 4) {
+            const uint4 y = __ldg(reinterpret_cast<const uint4*>(src));
+            w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
+          } else {
+            const uint2 y = __ldg(reinterpret_cast<const uint2*>(src));
+            w[0] = y.x, w[1] = y.y;
+          }
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const int grp = pl * 2 + i / 2;
+            const float2 p = __half22float2(__ldg(reinterpret_cast<const __half2*>(u + U::pair(false, tok, grp))));
+            uint4 v;
+            v.x = bf16_pair(kv4::centre_even(w[i]), p);
+            v.y = bf16_pair(kv4::centre_odd(w[i]), p);
+            v.z = bf16_pair(kv4::centre_even(w[i] >> 8), p);
+            v.w = bf16_pair(kv4::centre_odd(w[i] >> 8), p);
+            *reinterpret_cast<uint4*>(a.k + out + tok * step + pl * 128 + 32 * i + 8 * t) = v;
+          }
+        }
+    }
+    if (a.v) {
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int grp = 0; grp < GR; ++grp) {
+        const uint4 y = __ldg(reinterpret_cast<const uint4*>(u + U::kCodes + grp * 512 + lane * 16));
+        const uint32_t w[2][2] = {{y.x, y.y}, {y.z, y.w}};  // [32 dims][8 tokens]
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int tok = 8 * hh + 2 * t;
+          const float2 p0 = __half22float2(__ldg(reinterpret_cast<const __half2*>(u + U::pair(true, tok, grp))));
+          const float2 p1 = __half22float2(__ldg(reinterpret_cast<const __half2*>(u + U::pair(true, tok + 1, grp))));
+#pragma unroll
+          for (int il = 0; il < 2; ++il) {
+            uint32_t c[4] = {kv4::centre_even(w[il][hh]), kv4::centre_odd(w[il][hh]), kv4::centre_even(w[il][hh] >> 8),
+                             kv4::centre_odd(w[il][hh] >> 8)};  // dims 0 .. 3 of both tokens
+            uint16_t* dst = a.v + out + tok * step + grp * 64 + 32 * il + 4 * g;
+            *reinterpret_cast<uint2*>(dst) =
+                make_uint2(bf16_pair(__byte_perm(c[0], c[1], 0x5410), p0), bf16_pair(__byte_perm(c[2], c[3], 0x5410), p0));
+            *reinterpret_cast<uint2*>(dst + step) =
+                make_uint2(bf16_pair(__byte_perm(c[0], c[1], 0x7632), p1), bf16_pair(__byte_perm(c[2], c[3], 0x7632), p1));
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int64_t slot = __shfl_sync(0xffffffffu, mine, i);
+      const int64_t out = ((i0 + i) * a.nkv + h) * HD;
+#pragma unroll 1
+      for (int d = 4 * lane; d < HD; d += 128) {
+        uint2 k = make_uint2(0u, 0u), v = k;
+        if (slot >= 0 && slot < pool) {
+          const int off = (int)(slot % a.block_size), tok = off & 15;
+          const uint8_t* u =
+              a.cache + (((slot / a.block_size) * a.nkv + h) * (a.block_size / 16) + off / 16) * U::kBytes;
+          const uint32_t kw = *reinterpret_cast<const uint32_t*>(u + U::key_word(tok, d & ~7)) >> ((d & 4) * 2);
+          const uint32_t vw = *reinterpret_cast<const uint16_t*>(u + U::value_half(tok, d));
+          const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(u + U::pair(false, tok, d >> 6)));
+          const float2 vp = __half22float2(*reinterpret_cast<const __half2*>(u + U::pair(true, tok, d >> 6)));
+          k = make_uint2(bf16_pair(kv4::centre_even(kw), kp), bf16_pair(kv4::centre_odd(kw), kp));
+          const uint32_t c[4] = {kv4::centre_even(vw), kv4::centre_odd(vw), kv4::centre_even(vw >> 8), kv4::centre_odd(vw >> 8)};
+          v = make_uint2(bf16_pair(__byte_perm(c[0], c[1], 0x5410), vp), bf16_pair(__byte_perm(c[2], c[3], 0x5410), vp));
+        }
+        if (a.k) *reinterpret_cast<uint2*>(a.k + out + d) = k;
+        if (a.v) *reinterpret_cast<uint2*>(a.v + out + d) = v;
+      }
     }
   }
-  auto put = [&](uint16_t* dst, const float (&x)[4]) {
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-    *reinterpret_cast<uint2*>(dst + th * HD + d) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-  };
-  if (a.k) put(a.k, k);
-  if (a.v) put(a.v, v);
   pdl_launch();
 }
 
@@ -330,23 +452,28 @@ void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl) {
   launch(kv4_plan_kernel, dim3(grid), dim3(kPlanThreads), smem, s, pdl, a);
 }
 
+template <int HD, int HB>
+static void launch_append(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {
+  const int per_warp = (HD == 64 ? 2 : 1) * HB, warps = (a.nh + 2 * a.nkv + per_warp - 1) / per_warp;
+  launch(kv4_append_kernel<HD, HB>, dim3(a.R, (warps + 3) / 4), dim3(128), 0, s, pdl, a);
+}
+
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {
   if (a.R <= 0) return;
-  const int hpw = a.hd == 64 ? 2 : 1, heads = a.nh + 2 * a.nkv;
-  const int64_t units = (int64_t)a.R * ((heads + hpw - 1) / hpw);
-  const dim3 grid((unsigned)((units + 7) / 8));
+  // several heads per warp once one head per warp would fill the SMs twice over
+  const bool many = (int64_t)a.R * (a.nh + 2 * a.nkv) >= 148 * 64 * 2;
   switch (a.hd) {
-    case 64: launch(kv4_append_kernel<64>, grid, dim3(256), 0, s, pdl, a); break;
-    case 128: launch(kv4_append_kernel<128>, grid, dim3(256), 0, s, pdl, a); break;
-    case 256: launch(kv4_append_kernel<256>, grid, dim3(256), 0, s, pdl, a); break;
+    case 64: many ? launch_append<64, 4>(a, s, pdl) : launch_append<64, 1>(a, s, pdl); break;
+    case 128: many ? launch_append<128, 4>(a, s, pdl) : launch_append<128, 1>(a, s, pdl); break;
+    case 256: many ? launch_append<256, 2>(a, s, pdl) : launch_append<256, 1>(a, s, pdl); break;
     default: throw std::runtime_error("kv4 append: head_dim 64, 128 or 256");
   }
 }
 
 void kv4_gather_launch(const Kv4GatherArgs& a, cudaStream_t s, bool pdl) {
   if (a.N <= 0) return;
-  const int64_t n = (int64_t)a.N * a.nkv * (a.hd / 4);
-  const dim3 grid((unsigned)((n + 255) / 256));
+  const int64_t tasks = (int64_t)((a.N + 15) / 16) * a.nkv;
+  const dim3 grid((unsigned)((tasks + 7) / 8), 2);
   switch (a.hd) {
     case 64: launch(kv4_gather_kernel<64>, grid, dim3(256), 0, s, pdl, a); break;
     case 128: launch(kv4_gather_kernel<128>, grid, dim3(256), 0, s, pdl, a); break;

@@ -32,6 +32,8 @@
 namespace hk {
 namespace {
 
+using kv4::centre_even;
+using kv4::centre_odd;
 using kv4::Unit;
 using sm100::smem_u32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -63,21 +65,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// centred codes of the even (0x000f000f) and odd (0x00f000f0) nibbles as float16 pairs
-__device__ __forceinline__ uint32_t centre_even(uint32_t w) {
-  const uint32_t x = (w & 0x000f000fu) | 0x64006400u;  // 1024 + m
-  const uint32_t k = 0xe408e408u;                      // -1032
-  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&k));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t centre_odd(uint32_t w) {
-  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u;              // 1024 + 16 m
-  const uint32_t s = 0x2c002c00u, k = 0xd480d480u;                 // 1 / 16, -72
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&s),
-                            *reinterpret_cast<const __half2*>(&k));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // Loads past the L1 cache, of shared or global memory, that may be in flight together.
 __device__ __forceinline__ float2 fresh2(const float* p) {
   float2 v;

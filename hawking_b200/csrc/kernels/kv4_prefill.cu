@@ -100,12 +100,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ __half2 as_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-// (code - 8) s + c of the even (0x000f000f) and odd (0x00f000f0) nibble pairs of w
+// (code - 8) s + c of the even and odd nibble pairs of w
 __device__ __forceinline__ uint32_t value_even(uint32_t w, __half2 s, __half2 c) {
-  return as_u32(__hfma2(__hadd2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0xe408e408u)), s, c));
+  return as_u32(__hfma2(as_h2(kv4::centre_even(w)), s, c));
 }
 __device__ __forceinline__ uint32_t value_odd(uint32_t w, __half2 s, __half2 c) {
-  return as_u32(__hfma2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u), as_h2(0xd480d480u)), s, c));
+  return as_u32(__hfma2(as_h2(kv4::centre_odd(w)), s, c));
 }
 
 #define HK_R4(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3])

@@ -95,8 +95,8 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[torc
     position to). A row with a negative or foreign slot stores nothing, a row with a position
     outside ``rope`` is left alone.
 
-    Groups of 64 dims: s = f16((max - min) / 15), c = f16(min + 8 s), code = rint((x - c) / s) + 8
-    in 0..15, each operation in fp32. Finite values beyond +-65024 are clamped to it; a group with
+    Groups of 64 dims: s = f16((max - min) * (1 / 15)), c = f16(min + 8 s), code =
+    rint((x - c) / s) + 8 in 0..15 (8 where s is 0), each operation rounded to fp32. Finite values beyond +-65024 are clamped to it; a group with
     a NaN or an infinity reads back as NaN."""
     launches.add()
     kernels().kv4_append(qkv, positions, slots, rope, rot_dim, style, q_out, cache, nh, nkv, hd, bias, q_norm, k_norm,

@@ -298,7 +298,7 @@ def _pack_pairs(x):
     """The documented quantiser in fp32: (values that the codes stand for, s, c), float64."""
     g = x.float().reshape(*x.shape[:-1], -1, 64).clamp(-65024, 65024)
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s = ((hi - lo) / torch.full_like(hi, 15.0)).half().float()  # (by a Python number torch multiplies by 1 / 15)
+    s = ((hi - lo) * torch.full_like(hi, 1.0 / 15.0)).half().float()
     c = (lo + 8.0 * s).half().float()
     code = torch.where(s > 0, torch.round((g - c) / s) + 8, torch.full_like(g, 8)).clamp(0, 15)
     return (c.double() + s.double() * (code.double() - 8)).reshape(x.shape), s.double(), c.double()

@@ -27,6 +27,8 @@ def _cmd_generate(a) -> int:
     from .engine.sampling import SamplingParams
     from .config import runtime_profile
     extra = {k: v for k, v in runtime_profile(a.profile).engine.items() if k != "max_batch"}
+    if a.kv_bits != 16:
+        extra["kv_bits"] = a.kv_bits
     if a.gguf:
         from .engine.engine import Engine
         eng = Engine.from_gguf(a.gguf, max_batch=1, max_ctx=a.max_ctx, **extra)
@@ -37,6 +39,9 @@ def _cmd_generate(a) -> int:
     else:
         from .serve.__main__ import preset_engine
         eng, tok = preset_engine(a.preset, a.layers, 1, a.max_ctx, **extra)
+    if getattr(eng.kv, "bits", 16) != a.kv_bits:
+        print(f"--kv-bits {a.kv_bits}: not available for this model's cache", file=sys.stderr)
+        return 2
     eng.apply_profile(a.profile)
     ids = tok.encode(a.prompt, True)
     p = SamplingParams(temperature=a.temperature, top_p=a.top_p, top_k=a.top_k, seed=a.seed, max_tokens=a.max_tokens,
@@ -203,6 +208,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     g.add_argument("--seed", type=int, default=42)
     g.add_argument("--json", action="store_true")
     g.add_argument("--profile", default="default", help="runtime profile: default, fast, race, efficient, exact")
+    g.add_argument("--kv-bits", type=int, default=16, choices=(16, 4),
+                   help="KV cache precision of the Llama / Qwen / Mixtral families: 16 (bf16) or 4")
     g.add_argument("--stats", action="store_true", help="print the engine's stats JSON to stderr")
     t = sub.add_parser("tokenize", help="text <-> token ids")
     t.add_argument("--gguf", required=True)

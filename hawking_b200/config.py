@@ -58,6 +58,7 @@ class EngineConfig:
     max_prefill_tokens: int = 512      # prompt tokens per scheduler step (chunked prefill)
     kv_fraction: float = 0.5           # share of free device memory for the KV pool
     policy: int = 0                    # 0 default, 1 greedy-first, 2 prefix-grouped
+    kv_bits: int = 16                  # KV cache precision: 16 (bf16) or 4
 
     def build_kwargs(self) -> dict:
         return asdict(self)

@@ -9,7 +9,9 @@ corrupt or truncated file is refused, never half-loaded).
 
 File layout (little endian): b"HKKVSNP1" | u32 header_len | canonical JSON header | payload.
 The header holds the token ids, the cache geometry (layers, kv heads, head dim, dtype) and the
-payload digest; the payload is K then V, each [n_tokens, layers, kv_heads, head_dim] bf16.
+payload digest; the payload is K then V, each [n_tokens, layers, kv_heads, head_dim] bf16. A cache in 4 bits
+is written as its blocks' bytes (dtype "kv4", [layers, blocks, ...]) and restored bit for bit into blocks of
+the same size.
 
 ``PrefixDiskCache`` keeps such snapshots in a directory keyed by the rolling SHA-256 of the token
 prefix and finds the longest cached prefix of a new prompt (LRU by file time, bounded count).
@@ -84,6 +86,15 @@ def save_sequence(kv, seq_id: int, tokens: Sequence[int], path: str) -> dict:
     n = len(tokens)
     if kv.bm.num_tokens(seq_id) < n:
         raise ValueError("sequence holds fewer cached tokens than requested")
+    if getattr(kv, "bits", 16) == 4:
+        blocks = torch.tensor(kv.bm.table(seq_id)[: -(-n // kv.block_size)], dtype=torch.int64, device=kv.device)
+        payload = kv.data[:, blocks].contiguous().cpu().numpy().tobytes()
+        header = {"schema": "hawking_b200.kv_snapshot.v1", "tokens": [int(t) for t in tokens],
+                  "layers": kv.layers, "kv_heads": kv.nkv, "head_dim": kv.hd, "dtype": "kv4",
+                  "block_size": kv.block_size, "payload_bytes": len(payload),
+                  "payload_sha256": hashlib.sha256(payload).hexdigest()}
+        _atomic_write(path, MAGIC_KV, header, payload)
+        return header
     slots = _token_slots(kv, seq_id, n)
     k = _gather(kv.k, slots, kv.block_size).contiguous().cpu()
     v = _gather(kv.v, slots, kv.block_size).contiguous().cpu()
@@ -100,10 +111,19 @@ def load_sequence(kv, seq_id: int, path: str) -> List[int]:
     header, payload = _read(path, MAGIC_KV)
     if (header["layers"], header["kv_heads"], header["head_dim"]) != (kv.layers, kv.nkv, kv.hd):
         raise ValueError("snapshot geometry does not match this cache")
+    four = getattr(kv, "bits", 16) == 4
+    if header["dtype"] != ("kv4" if four else "bf16") or (four and header["block_size"] != kv.block_size):
+        raise ValueError("snapshot precision or block size does not match this cache")
     tokens = header["tokens"]
     n = len(tokens)
     if not kv.bm.reserve(seq_id, n):
         raise RuntimeError("KV pool exhausted while restoring a snapshot")
+    if four:
+        blocks = torch.tensor(kv.bm.table(seq_id)[: -(-n // kv.block_size)], dtype=torch.int64, device=kv.device)
+        raw = torch.frombuffer(bytearray(payload), dtype=torch.uint8) if payload else torch.empty(0, dtype=torch.uint8)
+        kv.data[:, blocks] = raw.view(kv.layers, len(blocks), *kv.data.shape[2:]).to(kv.device)
+        kv.sync_tables([seq_id])
+        return tokens
     shape = (n, kv.layers, kv.nkv, kv.hd)
     half = len(payload) // 2
     k = torch.frombuffer(bytearray(payload[:half]), dtype=torch.bfloat16).view(shape).to(kv.k.device)

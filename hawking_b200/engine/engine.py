@@ -27,7 +27,7 @@ from .._ext import native
 from ..config import check_memory_budget, env_flag
 from ..models.config import ModelConfig
 from ..utils.trace import trace
-from .kv_cache import PagedKVCache
+from .kv_cache import PagedKV4Cache, PagedKVCache
 from .sampling import RequestRng, SamplingParams
 
 
@@ -85,7 +85,8 @@ class Engine:
         # tensor-parallel collectives' peer waits): a nonzero word fails the step before any of
         # its tokens are committed
         self._status_dev = [t for t in (getattr(model, "status", None),
-                                        getattr(getattr(model, "tp", None), "status", None)) if t is not None]
+                                        getattr(getattr(model, "tp", None), "status", None),
+                                        getattr(getattr(kv, "ws", None), "status", None)) if t is not None]
         self._host_status = torch.zeros(max(1, len(self._status_dev)), dtype=torch.int32).pin_memory()
         self.tokenizer = None  # token bytes for JSON-mode requests (set by the server)
         # per-step cost ledger (HK_LEDGER=1 or ledger=True): host phases of every step, in us
@@ -100,15 +101,21 @@ class Engine:
     @staticmethod
     def build(cfg: ModelConfig, weights, device="cuda", max_batch: int = 8, max_ctx: Optional[int] = None,
               block_size: int = 64, num_blocks: Optional[int] = None, max_rows: int = 64,
-              max_prefill_tokens: int = 512, kv_fraction: float = 0.5, policy: int = 0, tp=None):
-        """``tp`` (parallel.tp.TPComm): ``cfg`` and ``weights`` are this rank's tensor-parallel shard."""
+              max_prefill_tokens: int = 512, kv_fraction: float = 0.5, policy: int = 0, tp=None, kv_bits: int = 16):
+        """``tp`` (parallel.tp.TPComm): ``cfg`` and ``weights`` are this rank's tensor-parallel shard.
+        ``kv_bits`` 4 holds the KV cache in 4 bits (engine/kv_cache.py PagedKV4Cache).
+
+        Parity: workspace/docs/reference/env_flags.md:29-35 (the int4 KV mode)."""
         from ..models.llama import LlamaModel
         max_ctx = max_ctx or cfg.max_ctx
         if cfg.is_moe and tp is None:
             # MoE prefill decodes every expert once per forward (grouped tensor-core GEMMs):
             # prompts run in forwards of up to 2048 rows so that cost is shared by more tokens
             max_prefill_tokens = max(max_prefill_tokens, 2048)
-        bpb = PagedKVCache.bytes_per_block(cfg.layers, cfg.n_kv_heads, cfg.head_dim, block_size)
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, not {kv_bits}")
+        cache = PagedKV4Cache if kv_bits == 4 else PagedKVCache
+        bpb = cache.bytes_per_block(cfg.layers, cfg.n_kv_heads, cfg.head_dim, block_size)
         free, _ = torch.cuda.mem_get_info(device)
         if num_blocks is None:
             num_blocks = int(free * kv_fraction // bpb)
@@ -117,8 +124,8 @@ class Engine:
         check_memory_budget(max(num_blocks, -(-max_ctx // block_size)) * bpb, free,
                             f"paged KV pool ({num_blocks} blocks of {block_size} tokens)", reserve_bytes=0)
         # one block-table row beyond max_batch: scratch sequences (embeddings) never starve
-        kv = PagedKVCache(cfg.layers, cfg.n_kv_heads, cfg.head_dim, num_blocks, block_size, max_batch + 1,
-                          -(-max_ctx // block_size), device)
+        kv = cache(cfg.layers, cfg.n_kv_heads, cfg.head_dim, num_blocks, block_size, max_batch + 1,
+                   -(-max_ctx // block_size), device)
         # one forward holds a whole prefill budget (the tensor-core GEMMs and prefill attention
         # want long row runs)
         model = LlamaModel(cfg, weights, kv, max_rows=max(max_rows, max_batch, max_prefill_tokens), device=device,
@@ -377,6 +384,9 @@ class Engine:
         if k <= 0:
             self.spec = None
             return
+        if getattr(self.kv, "bits", 16) == 4:
+            # its attention cuts the batch's keys into equal ranges: a row's rounding depends on the batch
+            raise ValueError("speculative decoding needs the 16-bit KV cache (its output is bitwise the greedy output)")
         n = native()
         self.spec = {"k": max(1, min(k, n.MAX_VERIFY_BATCH - 1, m.max_rows - 1)),
                      "gov": n.SpecGovernor(16, min_accept_rate), "drafts": {}, "cycles": 0, "drafted": 0,
@@ -521,6 +531,9 @@ class Engine:
         serial = getattr(m, "serial_rows", False)
         R = getattr(m, "row_limit", m.max_rows)
         per_item = []
+        kv4 = getattr(m, "kv4", False)
+        if kv4:  # single rows first: the decode kernel takes them together (the sort keeps the order otherwise)
+            items = sorted(items, key=lambda it: it.p1 - it.p0 > 1)
         for it in items:
             toks = self.sched.tokens(it.id)
             r = self.kv.row(it.id)
@@ -561,6 +574,7 @@ class Engine:
         decode_only = all(it.p1 - it.p0 == 1 for it in items)
         if hasattr(m, "long_runs"):
             m.long_runs = max((it.p1 - it.p0 for it in items), default=0) >= 16
+        singles = sum(it.p1 - it.p0 == 1 for it in items) if kv4 else 0
         greedy = all(it.greedy for it, _ in sample_rows)
         mode = "greedy" if greedy else "none"
         sampled: List[int] = []
@@ -568,7 +582,15 @@ class Engine:
         t_fwd = t_smp = 0.0
         for c0, c1 in bounds:
             ta = time.perf_counter()
-            self.stats.h2d_bytes += m.inp.upload(ids[c0:c1], pos[c0:c1], slots[c0:c1], rseq[c0:c1], rctx[c0:c1])
+            if kv4:
+                # the step's rows follow on the GPU from each request's lengths (one entry per run of rows)
+                runs = [k for k in range(c0, c1) if k == c0 or rseq[k] != rseq[k - 1]]
+                ends = runs[1:] + [c1]
+                m.decode_rows = max(0, min(singles, c1) - c0)
+                self.stats.h2d_bytes += m.inp.upload_plan(ids[c0:c1], [(rseq[a], pos[a], b - a) for a, b in zip(runs, ends)],
+                                                          self.kv, self.kv.ws.status)
+            else:
+                self.stats.h2d_bytes += m.inp.upload(ids[c0:c1], pos[c0:c1], slots[c0:c1], rseq[c0:c1], rctx[c0:c1])
             rows_here = [(it, r - c0) for it, r in sample_rows if c0 <= r < c1]
             with trace("forward"):
                 if self.use_graphs and decode_only and c1 - c0 == n:
@@ -594,9 +616,9 @@ class Engine:
                     sampled.extend(self._sample(picks, greedy))
             t_smp += time.perf_counter() - tb
         self._check_device_status()
-        if serial and sample_rows:  # back to the plan's item order (rows ran in wave order)
+        if (serial or kv4) and sample_rows:  # back to the plan's item order (rows ran in another)
             by_id = {it.id: tok for (it, _), tok in zip(sample_rows, sampled)}
-            sampled = [by_id[it.id] for it in items if it.id in by_id]
+            sampled = [by_id[it.id] for it in plan.items if it.id in by_id]
         events = self.sched.commit(plan, sampled)
         now = time.perf_counter()
         out = []
@@ -649,6 +671,8 @@ class Engine:
             t.zero_()
         from ..ops import mg
         mg.MgScratch.get(self.model.dev).reset()
+        if getattr(self.kv, "ws", None) is not None:
+            self.kv.ws.reset()
         if getattr(self.model, "dstep", None) is not None:
             self.model.dstep.reset()
 

@@ -1,8 +1,9 @@
 """Paged KV cache storage on the device.
 
-One bf16 tensor per K and V: [layers, num_blocks, n_kv_heads, block_size, head_dim]. A block holds
-``block_size`` consecutive tokens of one sequence; each head's tokens inside a block are contiguous
-so the decode kernel reads whole rows. Block allocation, prefix sharing and copy-on-write live in
+``PagedKVCache``: one bf16 tensor per K and V, [layers, num_blocks, n_kv_heads, block_size, head_dim].
+A block holds ``block_size`` consecutive tokens of one sequence; each head's tokens inside a block are
+contiguous so the decode kernel reads whole rows. ``PagedKV4Cache``: the same pool in 4 bits (ops/kv4.py),
+one uint8 tensor at 9/32 of the bytes. Block allocation, prefix sharing and copy-on-write live in
 the C++ ``BlockManager``; this class owns the memory and the device-side block tables.
 """
 from __future__ import annotations
@@ -15,6 +16,8 @@ from .._ext import native
 
 
 class PagedKVCache:
+    bits = 16
+
     def __init__(self, layers: int, n_kv_heads: int, head_dim: int, num_blocks: int, block_size: int,
                  max_seqs: int, max_blocks_per_seq: int, device, prefix_cache: bool = True,
                  dtype=torch.bfloat16):
@@ -22,8 +25,7 @@ class PagedKVCache:
             raise ValueError("KV pool too large for int32 slot ids")
         self.layers, self.nkv, self.hd = layers, n_kv_heads, head_dim
         self.num_blocks, self.block_size = num_blocks, block_size
-        self.k = torch.zeros(layers, num_blocks, n_kv_heads, block_size, head_dim, dtype=dtype, device=device)
-        self.v = torch.zeros_like(self.k)
+        self._allocate(device, dtype)
         self.max_seqs, self.max_blocks = max_seqs, max_blocks_per_seq
         self.block_tables = torch.zeros(max_seqs, max_blocks_per_seq, dtype=torch.int32, device=device)
         self._host_tables = torch.zeros(max_seqs, max_blocks_per_seq, dtype=torch.int32).pin_memory() \
@@ -32,6 +34,14 @@ class PagedKVCache:
         self._row_of: Dict[int, int] = {}
         self._free_rows: List[int] = list(range(max_seqs - 1, -1, -1))
         self._synced_len: Dict[int, int] = {}
+
+    def _allocate(self, device, dtype):
+        self.k = torch.zeros(self.layers, self.num_blocks, self.nkv, self.block_size, self.hd, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+
+    @property
+    def device(self) -> torch.device:
+        return self.block_tables.device
 
     @staticmethod
     def bytes_per_block(layers: int, n_kv_heads: int, head_dim: int, block_size: int, elem_bytes: int = 2) -> int:
@@ -73,3 +83,37 @@ class PagedKVCache:
         for src, dst in pairs:
             self.k[:, dst].copy_(self.k[:, src])
             self.v[:, dst].copy_(self.v[:, src])
+
+
+class PagedKV4Cache(PagedKVCache):
+    """The pool in 4 bits: ``data`` is uint8 [layers, num_blocks, n_kv_heads, block_size / 16,
+    18 * head_dim] (ops/kv4.py describes a unit), ``ws`` what the attention launches share. The block
+    size is a multiple of 16, the head dim 64, 128 or 256."""
+
+    bits = 4
+
+    def _allocate(self, device, dtype):
+        from ..ops import kv4
+        shape = kv4.cache_shape(self.num_blocks, self.nkv, self.block_size, self.hd)
+        self.data = torch.zeros(self.layers, *shape, dtype=torch.uint8, device=device)
+        self.ws = kv4.Workspace(device)
+
+    @staticmethod
+    def bytes_per_block(layers: int, n_kv_heads: int, head_dim: int, block_size: int, elem_bytes: int = 2) -> int:
+        from ..ops import kv4
+        return layers * n_kv_heads * (block_size // 16) * kv4.unit_bytes(head_dim)
+
+    def copy_blocks(self, pairs: List[Tuple[int, int]]):
+        for src, dst in pairs:
+            self.data[:, dst].copy_(self.data[:, src])
+
+    def read(self, seq_id: int, layer: int, n: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The first ``n`` (default: all) cached tokens' keys and values of one layer, as bf16
+        [n, n_kv_heads, head_dim] rows: what attention reads, for a snapshot or a move to a 16-bit cache."""
+        from ..ops import kv4
+        n = self.bm.num_tokens(seq_id) if n is None else n
+        slots = torch.tensor(self.bm.slots(seq_id, 0, n), dtype=torch.int32, device=self.device)
+        k = torch.empty(n, self.nkv, self.hd, dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
+        kv4.gather(self.data[layer], slots, k, v)
+        return k, v

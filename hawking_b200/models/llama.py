@@ -28,7 +28,7 @@ from .. import ops
 from ..formats.ggml import GgmlType, type_id
 from ..formats.gguf import GgufModel
 from ..ops import Q8Act, QWeight, cat_rows
-from ..ops import mg
+from ..ops import kv4, mg
 from .config import ModelConfig
 
 GEMV_COLS = 8  # rows per GEMV launch (dp4a GEMV batch limit)
@@ -245,6 +245,30 @@ class StepInputs:
         self._host_done[i] = ev
         return n * 5 * 4
 
+    def upload_plan(self, ids, requests, kv, status) -> int:
+        """The rows of a step from its requests: ``requests`` lists (block-table row, tokens cached, new
+        tokens) in row order, ``ids`` the new tokens. Only these are copied to the device; positions, slots
+        and the rest follow there (ops/kv4.py plan_rows). Returns the bytes copied."""
+        n, s = len(ids), len(requests)
+        i = self._turn
+        self._turn ^= 1
+        if self._host_done[i] is not None:
+            self._host_done[i].synchronize()
+        h = self._host_ring[i]
+        h[0, :n] = torch.as_tensor(ids, dtype=torch.int32)
+        h[1:4, :s] = torch.as_tensor(requests, dtype=torch.int32).t()
+        if getattr(self, "_plan_dev", None) is None:
+            self._plan_dev = torch.zeros(3, self.ids.shape[0], dtype=torch.int32, device=self.ids.device)
+        self.ids[:n].copy_(h[0, :n], non_blocking=True)
+        self._plan_dev[:, :s].copy_(h[1:4, :s], non_blocking=True)
+        ev = self._host_done[i] or torch.cuda.Event()
+        ev.record()
+        self._host_done[i] = ev
+        seq_rows, cached, new = (t[:s] for t in self._plan_dev)
+        kv4.plan_rows(seq_rows, cached, new, kv.block_tables, kv.block_size, self.positions[:n], self.row_seq[:n],
+                      self.row_ctx[:n], self.slots[:n], status=status)
+        return 4 * (n + 3 * s)
+
 
 class LlamaModel:
     """Runs the forward over static buffers for up to ``max_rows`` rows."""
@@ -268,7 +292,13 @@ class LlamaModel:
         self.att = Q8Act(R, nh * hd, self.dev)
         self.hq = Q8Act(R, F, self.dev)
         self.qkv = torch.zeros(R, qkv_n, device=self.dev)
-        self.q = torch.zeros(R, nh, hd, device=self.dev)
+        # a cache in 4 bits (engine/kv_cache.py PagedKV4Cache): bf16 queries, and fp32 attention rows where
+        # the output projection takes int8 blocks
+        self.kv4 = getattr(kv, "bits", 16) == 4
+        self.q = torch.zeros(R, nh, hd, device=self.dev, dtype=torch.bfloat16 if self.kv4 else torch.float32)
+        self.attf = torch.zeros(R, nh * hd, device=self.dev) if self.kv4 else None
+        # rows at the front of a long_runs forward that are one token of a sequence each (4-bit cache)
+        self.decode_rows = 0
         cap = max(r * self.num_splits(r) for r in range(1, R + 1))
         self.part_o = torch.zeros(cap * nh * hd, device=self.dev)
         self.part_lse = torch.zeros(cap * nh, device=self.dev)
@@ -326,7 +356,7 @@ class LlamaModel:
         # bs <= 4 decode as one persistent launch: opt-in (HK_DSTEP=1); measured slower than the
         # per-kernel path on B200 so far (per-phase barrier, staging and K/V-ring latencies)
         self.dstep = None
-        if os.environ.get("HK_DSTEP", "0") == "1" and self.small_batch == "w4a16":
+        if os.environ.get("HK_DSTEP", "0") == "1" and self.small_batch == "w4a16" and not self.kv4:
             from ..ops.dstep import DecodeStep
             self.dstep = DecodeStep.build(self)
 
@@ -481,6 +511,9 @@ class LlamaModel:
     def _rope_attention(self, l, lw, rows, splits, out_q8=None, out_bf16=None, roped: bool = False):
         """RoPE + paged append (unless the QKV GEMV's epilogue did both: ``roped``), then attention."""
         cfg, kv, inp = self.cfg, self.kv, self.inp
+        if self.kv4:
+            self._rope_attention_kv4(l, lw, rows, out_q8, out_bf16)
+            return
         if not roped:
             ops.rope_append(self.qkv[:rows], inp.positions[:rows], None, self.rope, cfg.rope_dim,
                             cfg.rope_style, self.q[:rows], kv.k[l], kv.v[l], cfg.n_heads, cfg.n_kv_heads,
@@ -494,11 +527,30 @@ class LlamaModel:
                              inp.row_ctx[:rows], self.scale, splits, self.part_o, self.part_lse,
                              out_q8=out_q8, out_bf16=out_bf16, counters=self.attn_counters)
 
+    def _rope_attention_kv4(self, l, lw, rows, out_q8, out_bf16):
+        """RoPE + quantising append, then attention over the 4-bit cache: rows that are one token of a
+        sequence each by the decode kernel, runs of rows by the prefill kernel (head dims 64 and 128)."""
+        cfg, kv, inp = self.cfg, self.kv, self.inp
+        data, q = kv.data[l], self.q[:rows]
+        kv4.rope_append(self.qkv[:rows], inp.positions[:rows], None, self.rope, cfg.rope_dim, cfg.rope_style, q, data,
+                        cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, bias=lw.qkv_bias, q_norm=lw.q_norm,
+                        k_norm=lw.k_norm, eps=cfg.eps, block_tables=kv.block_tables, row_seq=inp.row_seq[:rows])
+        n = rows  # rows for the decode kernel
+        if self.long_runs and cfg.head_dim in kv4.PREFILL_HEAD_DIMS:
+            n = min(rows, self.decode_rows)
+        for fn, a, b in ((kv4.attention_decode, 0, n), (kv4.attention_prefill, n, rows)):
+            if a < b:
+                fn(q[a:b], data, kv.block_tables, inp.row_seq[a:b], inp.row_ctx[a:b], self.scale, kv.ws,
+                   out=self.attf[a:b] if out_q8 is not None else None,
+                   out_bf16=out_bf16[a:b] if out_bf16 is not None else None)
+        if out_q8 is not None:
+            ops.rmsnorm_q8(self.attf[:rows], None, 0.0, out_q8, norm=False)
+
     # ---- W4A16 small-batch path (ops/mg.py) ----
     def _rope_in_qkv(self, lw) -> bool:
         """RoPE and the paged append run in the QKV GEMV epilogue (QKV packed in RoPE-pair
         order, no per-head q/k norm, whose reduction spans the head; HK_ROPE_EPI=0 turns it off)."""
-        return ROPE_EPI and lw.mg_qkv is not None and lw.mg_qkv.rope is not None and lw.q_norm is None \
+        return ROPE_EPI and not self.kv4 and lw.mg_qkv is not None and lw.mg_qkv.rope is not None and lw.q_norm is None \
             and lw.k_norm is None
 
     def _rope_args(self, l, c0, c1):
@@ -812,7 +864,7 @@ class LlamaModel:
         r = kv.row(seq_id)
         out = torch.empty(n, self.logits.shape[1], device=self.dev)  # this rank's vocabulary slice under TP
         step = min(self.max_logit_rows, self.row_limit)
-        self.long_runs = True
+        self.long_runs, self.decode_rows = True, 0
         try:
             for c0 in range(0, n, step):
                 c1 = min(n, c0 + step)

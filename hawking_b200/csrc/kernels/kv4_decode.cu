@@ -39,7 +39,7 @@ using sm100::smem_u32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTree = 8;       // CTAs whose partials are merged first where a pair has more than kFlat
 constexpr int kFlat = 24;
-constexpr int kMinUnits = 8;   // units (and visits) of a warp below which fewer work
+constexpr int kMinUnits = 3;   // units (and visits) of a warp below which fewer work
 constexpr int kVisit = 4;      // what a pair costs a warp besides its units, in units
 constexpr float kHead = 7.f;   // log2 of how far a score may exceed the reference
 
@@ -123,7 +123,7 @@ struct PartList {
 template <int HD>
 __device__ __noinline__ void merge_parts(const Kv4AttnArgs& a, const PartList from, int n, int row, int head, int h,
                                          int d, int ml_in, float* dst, int ml_out) {
-  constexpr int kRow = HD + 4, kFly = 12;  // loads in flight
+  constexpr int kRow = HD + 4, kFly = 8;  // loads in flight
   float m = !dst && a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
   float lt = m > -INFINITY ? 1.f : 0.f;  // the sink's weight at reference m
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -214,10 +214,10 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     int sum = 0;
 #pragma unroll 1
     for (int r = r0; r < r1; ++r) {
-      const int seq = a.row_seq[r];
-      int len = min(max(a.row_ctx[r], 0), a.max_blocks * a.block_size);
-      if (seq < 0 || seq >= a.table_rows) {
-        len = 0;
+      int seq = a.row_seq[r];
+      const int len = min(max(a.row_ctx[r], 0), a.max_blocks * a.block_size);
+      if (seq < 0 || seq >= a.table_rows) {  // reads as zeros, and leaves the other rows' parts as they are
+        seq = -1;
         if (blockIdx.x == 0) set_error(a.status, HK_ERR_BAD_ARG);
       }
       rows[r] = make_int2(seq, len);
@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     const auto lookup = [&](bool pair) {
       if (pair) {
         head = a.cache + (int64_t)(cc.item >> g_.split) * upb * U::kBytes;
-        table = a.block_tables + (int64_t)rows[cc.row].x * a.max_blocks;
+        const int seq = rows[cc.row].x;
+        table = seq < 0 ? nullptr : a.block_tables + (int64_t)seq * a.max_blocks;
       }
       const int b0 = g_.upb_shift >= 0 ? cc.u >> g_.upb_shift : cc.u / upb;
       at = cc.u - b0 * upb;
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
         if (i > 0 && ++k == upb) k = 0, ++b;
         if (i == 0 && kept) blk[0] = blk_last;
         else if (i > 0 && b == b0) blk[i] = blk[0];
-        else if (cc.u + i < cc.units) blk[i] = table[b];
+        else if (cc.u + i < cc.units) blk[i] = table ? table[b] : -1;
       }
     };
     uint8_t* const my_ring = smem + lane * Sh::kRing;

@@ -115,8 +115,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
 
 // ---- RoPE + quantise + append ----------------------------------------------------------------------
 // A warp takes HB heads of one row (HB pairs of heads at HD 64), so that the position's rotation is read once
-// for them and all their loads are in flight together: at 2048 rows of 48 heads HB = 4 against 1 measured
-// FIG_HB; a few rows keep one head per warp (the launch needs warps more than the warps need work).
+// for them and all their loads are in flight together: at 2048 rows of 48 heads of 128 in the L2 cache HB = 4 took
+// 17 us, 2 took 21, 1 took 31. A few rows keep one head per warp (the launch needs warps more than the warps work).
 // Every lane holds 4 consecutive dims of each 128 (or 64), 16 lanes the 64 dims of a quantisation group.
 // Sums, products and divisions are rounded one by one, the norm's sum of squares in a fixed order,
 // so the bytes written do not depend on how the compiler contracts them.
@@ -128,7 +128,24 @@ __device__ __forceinline__ Vec4 ld4(const float* p) {
   return {{f.x, f.y, f.z, f.w}};
 }
 
-template <int HD, int HB>
+// minimum and maximum that keep a NaN
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <int HD, int HB, int STYLE, bool EXTRA>
 __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
   constexpr int LG = HD < 128 ? HD / 4 : 32;  // lanes of one head
   constexpr int HPW = 32 / LG;                // heads side by side in a warp
@@ -137,8 +154,8 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
   pdl_wait();
   const int lane = threadIdx.x & 31, sl = lane % LG;
   const int heads = a.nh + 2 * a.nkv, per_row = (heads + HPW * HB - 1) / (HPW * HB);
-  const int r = blockIdx.x, unit = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (unit >= per_row) return;
+  const int r = blockIdx.x, unit = (gridDim.y - 1 - blockIdx.y) * 4 + (threadIdx.x >> 5);
+  if (unit >= per_row) return;  // (the last heads, keys and values, first: they take longest)
   const int h0 = unit * (HPW * HB) + lane / LG;
   const float* row = a.qkv + (int64_t)r * a.qkv_stride;
   Vec4 x[HB][NV];
@@ -178,7 +195,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
       cs[j][e] = 1.f;
       sn[j][e] = 0.f;
       if (d < a.rot_dim) {
-        const int i = a.rope_style == 0 ? d >> 1 : (d < half ? d : d - half);
+        const int i = STYLE == 0 ? d >> 1 : (d < half ? d : d - half);
         const float2 t = *reinterpret_cast<const float2*>(rope + 2 * i);
         cs[j][e] = t.x;
         sn[j][e] = t.y;
@@ -191,8 +208,8 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
     const int hc = min(h, heads - 1);
     const int kind = hc < a.nh ? 0 : (hc < a.nh + a.nkv ? 1 : 2);  // q, k, v
     const float* src = row + (int64_t)hc * HD;
-    const float* bias = a.bias ? a.bias + (int64_t)hc * HD : nullptr;
-    const float* nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
+    const float* bias = EXTRA && a.bias ? a.bias + (int64_t)hc * HD : nullptr;
+    const float* nw = !EXTRA ? nullptr : kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
     Vec4(&v)[NV] = x[b];
     if (bias) {
 #pragma unroll
@@ -201,7 +218,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
         for (int e = 0; e < 4; ++e) v[j].v[e] = __fadd_rn(v[j].v[e], bias[128 * j + 4 * sl + e]);
     }
     float inv = 1.f;
-    if (a.q_norm || a.k_norm) {  // (the same for the warp)
+    if (EXTRA && (a.q_norm || a.k_norm)) {  // (the same for the warp)
       float ss[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -230,11 +247,24 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
           for (int e = 0; e < 4; ++e) v[j].v[e] = __fmul_rn(__fmul_rn(v[j].v[e], inv), nw[128 * j + 4 * sl + e]);
       }
     }
-    if (kind < 2) {
+    if (STYLE == 1 && a.rot_dim == HD) {  // pairs (d, d + half), in two lanes or in two vectors of one
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float y[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)  // (the two heads of a warp may be of two kinds: all lanes shuffle)
+          y[j] = NV == 1 ? __shfl_xor_sync(0xffffffffu, v[0].v[e], LG / 2) : v[NV - 1 - j].v[e];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const float p = __fmul_rn(v[j].v[e], cs[j][e]), q = __fmul_rn(y[j], sn[j][e]);
+          if (kind < 2) v[j].v[e] = 128 * j + 4 * sl < half ? __fsub_rn(p, q) : __fadd_rn(q, p);
+        }
+      }
+    } else if (kind < 2) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int d0 = 128 * j + 4 * sl;
-        if (a.rope_style == 0) {  // pairs (d, d + 1)
+        if (STYLE == 0) {  // pairs (d, d + 1)
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
             if (d0 + e < a.rot_dim) {
@@ -276,35 +306,46 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
     uint8_t* u = a.cache + (((int64_t)blk * a.nkv + kh) * (a.block_size / 16) + off / 16) * U::kBytes;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      bool odd = false;  // a NaN or an infinity in the group
-      float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float& t = v[j].v[e];
-        odd |= !(fabsf(t) < INFINITY);
-        t = fminf(fmaxf(t, -kv4::kMaxValue), kv4::kMaxValue);
-        lo = fminf(lo, t);
-        hi = fmaxf(hi, t);
-      }
+      float lo = min_nan(min_nan(v[j].v[0], v[j].v[1]), min_nan(v[j].v[2], v[j].v[3]));
+      float hi = max_nan(max_nan(v[j].v[0], v[j].v[1]), max_nan(v[j].v[2], v[j].v[3]));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
       }
-      odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 16) & 0xffffu) != 0;
+      const bool odd = !(lo > -INFINITY && hi < INFINITY);  // a NaN or an infinity in the group
+      if (lo < -kv4::kMaxValue || hi > kv4::kMaxValue) {
+        lo = fminf(fmaxf(lo, -kv4::kMaxValue), kv4::kMaxValue);
+        hi = fminf(fmaxf(hi, -kv4::kMaxValue), kv4::kMaxValue);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j].v[e] = fminf(fmaxf(v[j].v[e], -kv4::kMaxValue), kv4::kMaxValue);
+      }
       __half sh = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
       const float s = __half2float(sh);
       __half ch = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, s)));
       const float c = __half2float(ch);
+      // round((x - c) / s): by the reciprocal, whose product is off by less than 3e-6 where it matters (up to 8), and by
+      // the division where that product is within 1e-5 of a half. Adding kRound leaves code = round + 8 in the last bits.
+      constexpr float kRound = 12582912.f + 8.f;
+      const float rs = s > 0.f ? rcp(s) : 0.f;
       uint32_t code[4];
+      bool half_way = false;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float q = s > 0.f ? __fadd_rn(rintf(__fdiv_rn(__fsub_rn(v[j].v[e], c), s)), 8.f) : 8.f;
-        code[e] = odd ? 8u : (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
+        const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(v[j].v[e], c), rs), -8.f), 7.f);
+        const float t = __fadd_rn(q, kRound);
+        half_way |= fabsf(__fsub_rn(q, __fsub_rn(t, kRound))) > 0.49999f;
+        code[e] = __float_as_uint(t) & 15u;
       }
-      if (odd) sh = ch = __ushort_as_half(0x7fff);  // such a group reads back as NaN
+      if (half_way) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          code[e] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(v[j].v[e], c), s), -8.f), 7.f), kRound)) & 15u;
+      }
+      if (odd) sh = ch = __ushort_as_half(0x7fff);  // such a group reads back as NaN, its codes as 8
       // key words hold 8 dims: two lanes' parts
-      uint32_t w = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20;
+      uint32_t w = odd ? 0x00880088u : code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20;
+      const uint32_t vw = odd ? 0x8888u : code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12;
       w <<= (lane & 1) * 8;
       w |= __shfl_xor_sync(0xffffffffu, w, 1);
       if (store) {
@@ -312,8 +353,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
         if (kind == 1) {
           if ((lane & 1) == 0) *reinterpret_cast<uint32_t*>(u + U::key_word(tok, d)) = w;
         } else {
-          *reinterpret_cast<uint16_t*>(u + U::value_half(tok, d)) =
-              (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+          *reinterpret_cast<uint16_t*>(u + U::value_half(tok, d)) = (uint16_t)vw;
         }
         if ((lane & 15) == 0) *reinterpret_cast<__half2*>(u + U::pair(kind == 2, tok, d >> 6)) = __halves2half2(sh, ch);
       }
@@ -325,8 +365,9 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a) {
 // ---- gather ----------------------------------------------------------------------------------------
 // A warp takes 16 slots of one head. Where they are the 16 tokens of a unit in order, as a sequence's slots
 // are, it reads the unit whole, in its own order: a lane's 16 bytes of key codes are 4 x 8 dims of a token, its
-// 16 bytes of value codes 2 x 4 dims of four tokens, so loads and stores are whole sectors and a code costs
-// FIG_GATHER. Any other slots go token by token, 4 dims per lane.
+// 16 bytes of value codes 2 x 4 dims of four tokens, so loads and stores are whole sectors. 65536 slots of 8 heads
+// of 128 (344 MB, most of it written) took 60 us this way, 5.7 TB/s and bound by the memory; token by token, 4 dims
+// per lane, as any other slots go, 128 us.
 __device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, float2 p) {  // centred codes (float16 pair), (s, c)
   const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&codes));
   const __nv_bfloat162 v = __floats2bfloat162_rn(fmaf(p.x, n.x, p.y), fmaf(p.x, n.y, p.y));
@@ -455,7 +496,10 @@ void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl) {
 template <int HD, int HB>
 static void launch_append(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {
   const int per_warp = (HD == 64 ? 2 : 1) * HB, warps = (a.nh + 2 * a.nkv + per_warp - 1) / per_warp;
-  launch(kv4_append_kernel<HD, HB>, dim3(a.R, (warps + 3) / 4), dim3(128), 0, s, pdl, a);
+  const bool extra = a.bias || a.q_norm || a.k_norm;
+  const auto kernel = a.rope_style == 0 ? (extra ? kv4_append_kernel<HD, HB, 0, true> : kv4_append_kernel<HD, HB, 0, false>)
+                                        : (extra ? kv4_append_kernel<HD, HB, 1, true> : kv4_append_kernel<HD, HB, 1, false>);
+  launch(kernel, dim3(a.R, (warps + 3) / 4), dim3(128), 0, s, pdl, a);
 }
 
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {

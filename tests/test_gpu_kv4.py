@@ -344,6 +344,31 @@ def test_append_values_exact(nh, nkv, hd, style, part):
     assert (k.permute(0, 2, 1, 3)[rest] == 0).all() and (v.permute(0, 2, 1, 3)[rest] == 0).all()
 
 
+@pytest.mark.parametrize("rows,nh,nkv,hd", [(700, 32, 8, 128), (1500, 8, 3, 64), (2200, 7, 1, 64), (1000, 16, 2, 256)])
+@pytest.mark.parametrize("style,part", [(0, 1), (1, 1), (1, 2)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_append_many_rows_exact(rows, nh, nkv, hd, style, part, bias):
+    """Several heads per warp, and codes half way between two integers."""
+    g = torch.Generator(device=DEV).manual_seed(rows + style)
+    bs, rot = 16, hd // part
+    blocks = -(-rows // bs)
+    x = torch.randn(rows, nh + 2 * nkv, hd, device=DEV, generator=g)
+    x[:, nh + nkv:] = torch.randint(0, 31, (rows, nkv, hd), device=DEV, generator=g) / 2
+    b = torch.randint(-3, 4, ((nh + 2 * nkv) * hd,), device=DEV, generator=g).float() if bias else None
+    rope, pos = _rope(rows, rot), torch.arange(rows, dtype=torch.int32, device=DEV)
+    slots = torch.randperm(blocks * bs, device=DEV, generator=g)[:rows].int()
+    cache = torch.zeros(kv4.cache_shape(blocks, nkv, bs, hd), dtype=torch.uint8, device=DEV)
+    q = torch.empty(rows, nh, hd, dtype=torch.bfloat16, device=DEV)
+    kv4.rope_append(x.reshape(rows, -1), pos, slots, rope, rot, style, q, cache, nh, nkv, hd, bias=b)
+    if bias:
+        x = x + b.reshape(-1, hd)
+    turned = _rotate(x[:, :nh + nkv], rope, style, torch.float32)
+    assert torch.equal(q, turned[:, :nh].bfloat16())
+    s = slots.long()
+    for got, want in zip(_values(cache, hd), (turned[:, nh:], x[:, nh + nkv:])):
+        assert torch.equal(got[s // bs, :, s % bs], _pack_pairs(want)[0])
+
+
 @pytest.mark.parametrize("hd,rot,style", [(64, 64, 0), (128, 128, 1), (256, 64, 1)])
 def test_append_norm_against_64bit(hd, rot, style):
     g = torch.Generator(device=DEV).manual_seed(hd)

@@ -39,6 +39,7 @@ using sm100::smem_u32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTree = 8;       // CTAs whose partials are merged first where a pair has more than kFlat
 constexpr int kFlat = 24;
+constexpr int kMaxCtas = 32 * kTree;  // (a lane per partial)
 constexpr int kMinUnits = 3;   // units (and visits) of a warp below which fewer work
 constexpr int kVisit = 4;      // what a pair costs a warp besides its units, in units
 constexpr float kHead = 7.f;   // log2 of how far a score may exceed the reference
@@ -109,69 +110,84 @@ struct Part {
   int row, item, u0, u1;  // row < 0: none
 };
 
-// Partials in shared or global memory: number k, i = k + first, at (i % 2 ? odd : even) + (i / 2) stride, in
-// floats, the first one `lead` further on; bit k % 32 of live says whether there is one.
-struct PartList {
-  const float *even, *odd;
-  int first, even_stride, odd_stride, lead;
-  unsigned live;
+// Where a merged head goes: the output in either type, or a partial with its reference and sum at ml. Addresses,
+// so that nothing of the arguments is read again on the way.
+struct MergeTo {
+  float* part;
+  float2* ml;
+  uint16_t* out16;
+  float* out;
 };
 
-// Four dims d .. d + 3 of head h of the sum of n partials: to the output of the row's query head `head`
-// (with its sink), or to dst with the references and sums at ml_out (elsewhere than at ml_in if dst is
-// among the partials: other threads may still read those). Out of line: called in two places, runs cold.
-template <int HD>
-__device__ __noinline__ void merge_parts(const Kv4AttnArgs& a, const PartList from, int n, int row, int head, int h,
-                                         int d, int ml_in, float* dst, int ml_out) {
-  constexpr int kRow = HD + 4, kFly = 8;  // loads in flight
-  float m = !dst && a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
-  float lt = m > -INFINITY ? 1.f : 0.f;  // the sink's weight at reference m
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-  for (int k0 = 0; k0 < n; k0 += kFly) {
-    float2 ml[kFly];
-    float4 t[kFly];
+// One head of the sum of n <= 32 partials and of a sink of log2 weight m, if any, by a warp: lane k has the address of
+// partial k, in shared or global memory, where the head is `at` floats on and its reference and sum at `ml_at`. A lane
+// without a partial (live: false) has partial 0's address and weight 0. Every lane weighs one partial and sums 4 dims of
+// each 128. A few warps do this once, so what bounds it is the latency of its instructions, not the bytes: 11 partials of
+// 8 heads of 256 in shared memory took 4.4 us when a thread per 4 dims weighed all partials itself, 1.3 this way.
+template <int HD, int FLY>
+__device__ __noinline__ void merge_parts(const float* from, bool live, int n, int at, int ml_at, float m, const MergeTo to) {
+  constexpr int NV = (HD + 127) / 128;  // vectors of a lane; FLY: partials in flight
+  const int lane = threadIdx.x & 31;
+  const bool mine = HD >= 128 || lane < HD / 4;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (live) ml = fresh2(from + ml_at);
+  const unsigned long long base = reinterpret_cast<unsigned long long>(from + at);
+  const int d0 = HD >= 128 ? 4 * lane : 4 * (lane % (HD / 4));
+  float4 v[NV];
 #pragma unroll
-    for (int k = 0; k < kFly; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      t[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int i = k0 + k + from.first;
-      if (k0 + k < n && (from.live >> ((k0 + k) & 31) & 1)) {
-        const float* q = (i & 1 ? from.odd + (int64_t)(i >> 1) * from.odd_stride
-                                : from.even + (int64_t)(i >> 1) * from.even_stride) +
-                         (k0 + k ? 0 : from.lead) + h * kRow;
-        ml[k] = fresh2(q + ml_in);
-        t[k] = fresh4(q + d);
+  for (int j = 0; j < NV; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float e = 0.f, lt = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += FLY) {
+    float4 t[FLY][NV];
+#pragma unroll
+    for (int k = 0; k < FLY; ++k) {
+      const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, base, k0 + k)) + d0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) t[k][j] = fresh4(q + 128 * j);
+    }
+    if (k0 == 0) {
+      float top = fmaxf(m, ml.x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float mb = fmaxf(top, -1e30f);
+      e = ex2(ml.x - mb);
+      lt = ml.y * e;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+      lt += ex2(m - mb);  // the sink
+      m = top;
+    }
+#pragma unroll
+    for (int k = 0; k < FLY; ++k) {
+      const float w = __shfl_sync(0xffffffffu, e, k0 + k);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        v[j].x = fmaf(t[k][j].x, w, v[j].x), v[j].y = fmaf(t[k][j].y, w, v[j].y);
+        v[j].z = fmaf(t[k][j].z, w, v[j].z), v[j].w = fmaf(t[k][j].w, w, v[j].w);
       }
     }
-    float top = m;
-#pragma unroll
-    for (int k = 0; k < kFly; ++k) top = fmaxf(top, ml[k].x);
-    const float mb = fmaxf(top, -1e30f), f = ex2(m - mb);
-    m = top;
-    lt *= f;
-    v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-#pragma unroll
-    for (int k = 0; k < kFly; ++k) {
-      const float e = ex2(ml[k].x - mb);
-      v.x = fmaf(t[k].x, e, v.x), v.y = fmaf(t[k].y, e, v.y), v.z = fmaf(t[k].z, e, v.z), v.w = fmaf(t[k].w, e, v.w);
-      lt = fmaf(ml[k].y, e, lt);
-    }
   }
-  if (dst) {
-    __stcg(reinterpret_cast<float4*>(dst + h * kRow + d), v);
-    if (d == 0) __stcg(reinterpret_cast<float2*>(dst + h * kRow + ml_out), make_float2(m, lt));
+  if (to.part) {
+    if (mine)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) __stcg(reinterpret_cast<float4*>(to.part + 4 * lane + 128 * j), v[j]);
+    if (lane == 0) __stcg(to.ml, make_float2(m, lt));
     return;
   }
+  if (!mine) return;
   const float f = 1.f / lt;
-  v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-  const int64_t at = (int64_t)head * HD + d;
-  if (a.out_bf16) {
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2*>(a.out_bf16 + row * a.out_stride + at) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int d = 4 * lane + 128 * j;
+    const float4 z = make_float4(v[j].x * f, v[j].y * f, v[j].z * f, v[j].w * f);
+    if (to.out16) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(z.x, z.y), hi = __floats2bfloat162_rn(z.z, z.w);
+      *reinterpret_cast<uint2*>(to.out16 + d) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+    if (to.out) *reinterpret_cast<float4*>(to.out + d) = z;
   }
-  if (a.out) *reinterpret_cast<float4*>(a.out + row * a.outf_stride + at) = v;
 }
 
 template <int HD, int NT>
@@ -179,6 +195,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeArgs g_) {
   using U = Unit<HD>;
   using Sh = DecodeShape<HD, NT>;
+  static_assert(kFlat <= 32 && kTree <= 32, "one lane per partial");
   constexpr int GR = HD / 64, KT = HD / 16, TU = Sh::kTile, kWarps = Sh::kWarps, kThreads = Sh::kThreads,
                 kStages = Sh::kStages;
   const Kv4AttnArgs& a = g_.a;
@@ -694,6 +711,15 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     next_pair(cc);
   }
 
+  const auto sink_of = [&](const float* dst, int item, int h) {
+    return !dst && a.sinks ? a.sinks[head_of(item) + h] * kLog2e : -INFINITY;
+  };
+  const auto merge_to = [&](float* dst, int row, int item, int h, int ml_at) {
+    const int64_t at = (int64_t)(head_of(item) + h) * HD;
+    return MergeTo{dst ? dst + h * Sh::kRow : nullptr, reinterpret_cast<float2*>(dst + h * Sh::kRow + ml_at),
+                   a.out_bf16 ? a.out_bf16 + row * a.out_stride + at : nullptr,
+                   a.out ? a.out + row * a.outf_stride + at : nullptr};
+  };
   // ---- pairs that span warps or CTAs (rolled loops: this code runs once per CTA, cold) ----
   __syncthreads();
   // the CTA's pairs that reach into others: at most one at its begin (0) and one at its end (1)
@@ -707,13 +733,15 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     const int prev = below ? 31 - __clz(below) : lane;
     const int prow = __shfl_sync(0xffffffffu, p.row, prev), pitem = __shfl_sync(0xffffffffu, p.item, prev);
     const unsigned begins = __ballot_sync(0xffffffffu, p.row >= 0 && (!below || prow != p.row || pitem != p.item));
-    // all pairs at once: item x is four dims of one head of pair x / per
-    const int per = HPI * (HD / 4), work = __popc(begins) * per;
+    // all pairs at once: a warp takes one head of one pair, or finds the CTAs that a pair spans
+    const int pairs = __popc(begins), work = pairs * HPI;
 #pragma unroll 1
-    for (int x = tid; x < work; x += kThreads) {
+    for (int x = warp; x < work + pairs; x += kThreads / 32) {
+      const bool merges = x < work;
+      const int g = merges ? x / HPI : x - work, h = x - g * HPI;
       unsigned left = begins;
 #pragma unroll 1
-      for (int g = x / per; g > 0; --g) left &= left - 1;
+      for (int i = g; i > 0; --i) left &= left - 1;
       const int i0 = __ffs(left) - 1;
       const unsigned rest = left & (left - 1);
       const unsigned set = valid & ~((1u << i0) - 1) & (rest ? (rest & -rest) - 1 : ~0u);
@@ -723,11 +751,18 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
       const bool done = f.u0 == 0 && u1 == units;
       const int at0 = before[f.row] + f.item * (units + kVisit) + kVisit;  // place of its unit 0
       const int slot = at0 + f.u0 <= w0 ? 0 : 1;
-      float* dst = done ? nullptr : g_.part + ((int64_t)cta * 2 + slot) * pstride;
-      const PartList from{firsts, reinterpret_cast<const float*>(smem), i0, pstride, Sh::kRing / 4, 0, set >> i0};
-      const int y = x % per, h = y / (HD / 4), d = y % (HD / 4) * 4;
-      if (h < heads_of(f.item)) merge_parts<HD>(a, from, i1 - i0 + 1, f.row, head_of(f.item) + h, h, d, HD, dst, HD);
-      if (!done && y == 0) {
+      if (merges && h < heads_of(f.item)) {
+        float* dst = done ? nullptr : g_.part + ((int64_t)cta * 2 + slot) * pstride;
+        // a pair begins with its first warp's last partial and goes on in the next warps' last ones, the last
+        // warp's may be a first one; or it has but a first one
+        int i = i0 + 2 * lane;
+        if (i == i1 + 1) i = i1;
+        const bool live = i <= i1 && (set >> i & 1);
+        if (!live) i = i0;
+        const float* from = i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * Sh::kRing) : firsts + (i >> 1) * pstride;
+        merge_parts<HD, 4>(from, live, ((i1 | 1) - i0) / 2 + 1, h * Sh::kRow, h * Sh::kRow + HD, sink_of(dst, f.item, h),
+                           merge_to(dst, f.row, f.item, h, HD));
+      } else if (!merges && !done && lane == 0) {
         const int c0 = part_of(at0) / W;
         span[slot][1] = f.item;
         span[slot][2] = c0;
@@ -766,10 +801,9 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     __syncthreads();
     __threadfence();
     bool again = false;
-    const int per = HPI * (HD / 4);
 #pragma unroll 1
-    for (int x = tid; x < 2 * per; x += kThreads) {
-      const int s = x >= per ? 1 : 0;
+    for (int x = warp; x < 2 * HPI; x += kThreads / 32) {
+      const int s = x >= HPI ? 1 : 0;
       if (!last_s[s]) continue;
       const int row = span[s][0], item = span[s][1], c0 = span[s][2], n = span[s][3] - c0 + 1, first = span[s][4];
       const bool deep = n > kFlat, inner = deep && round == 0;
@@ -777,11 +811,14 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
       const int cnt = inner ? min(kTree, n - g0) : deep ? (n + kTree - 1) / kTree : n;
       float* part = g_.part + (int64_t)(c0 + g0) * 2 * pstride;
       const int off = g0 == 0 ? first * pstride : 0;
-      const PartList from{part, part + 2 * step * pstride, 0, 4 * step * pstride, 4 * step * pstride, off, ~0u};
-      const int y = x - s * per, h = y / (HD / 4), d = y % (HD / 4) * 4;
-      if (h < heads_of(item))
-        merge_parts<HD>(a, from, cnt, row, head_of(item) + h, h, d, deep && round ? HD + 2 : HD,
-                        inner ? part + off : nullptr, HD + 2);
+      const bool live = lane < cnt;
+      const float* from = part + (live && lane ? lane * 2 * step * pstride : off);
+      const int h = x - s * HPI;
+      if (h < heads_of(item)) {  // a sum's reference and sum go beside the first partial's: others still read those
+        float* dst = inner ? part + off : nullptr;
+        merge_parts<HD, 8>(from, live, cnt, h * Sh::kRow, h * Sh::kRow + (deep && round ? HD + 2 : HD), sink_of(dst, item, h),
+                        merge_to(dst, row, item, h, HD + 2));
+      }
     }
     for (int s = 0; s < 2; ++s) again |= last_s[s] && round == 0 && span[s][3] - span[s][2] + 1 > kFlat;
     if (!again) break;
@@ -801,7 +838,7 @@ void launch_decode(const DecodeArgs& d, int sms, cudaStream_t s, bool pdl) {
                                        Sh::kSmem));
     configured = true;
   }
-  launch(kv4_decode_kernel<HD, NT>, dim3(sms), dim3(Sh::kThreads), Sh::kSmem, s, pdl, d);
+  launch(kv4_decode_kernel<HD, NT>, dim3(std::min(sms, kMaxCtas)), dim3(Sh::kThreads), Sh::kSmem, s, pdl, d);
 }
 
 }  // namespace

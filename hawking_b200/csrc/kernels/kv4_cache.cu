@@ -504,8 +504,9 @@ static void launch_append(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {
 
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl) {
   if (a.R <= 0) return;
-  // several heads per warp once one head per warp would fill the SMs twice over
-  const bool many = (int64_t)a.R * (a.nh + 2 * a.nkv) >= 148 * 64 * 2;
+  // several heads per warp once one head each would make 80 warps per SM: 256 rows of 48 heads of 128 took 6.5 us with 4
+  // heads per warp and 6.6 with one, 384 rows 6.5 and 8.6, 128 rows 6.4 and 5.9
+  const bool many = (int64_t)a.R * (a.nh + 2 * a.nkv) >= 148 * 80;
   switch (a.hd) {
     case 64: many ? launch_append<64, 4>(a, s, pdl) : launch_append<64, 1>(a, s, pdl); break;
     case 128: many ? launch_append<128, 4>(a, s, pdl) : launch_append<128, 1>(a, s, pdl); break;

@@ -18,12 +18,23 @@
 // score exceeds it by 2^7 (weights of up to 128 are fine in float16): one vote per tile instead of a
 // reduction, and every lane sums its own tokens' weights until the end of a segment.
 //
-// Work. The (row, kv head) pairs' units of 16 tokens form one sequence that is cut into equal ranges,
+// More than 8 query heads per kv head make two items of it. (One item of two narrow tiles, which unpacks every code
+// once, was 7 % faster for 64 rows of 8000 tokens and 16 heads, but its registers halve the warps: 28 us against 20
+// for 8 such rows.)
+//
+// Work. The (row, item) pairs' units of 16 tokens form one sequence that is cut into equal ranges,
 // one per CTA (at least kMinUnits long), and each range into equal parts, one per warp: ragged batches
 // and single long rows load every warp alike, and a warp needs nobody inside its part. A pair that lies
 // in one part is written out by its warp; one that spans warps is merged in shared memory at the end
 // of the CTA; one that spans CTAs leaves partials (reference, sum, output), merged in CTA order by the
-// last CTA to arrive (groups of kTree CTAs first, where there are many).
+// last CTA to arrive (groups of kTree CTAs first, where there are many). One CTA per SM; a warp of it
+// only issues the copies for all others (bulk copies of whole units, a ring of tiles per warp).
+//
+// What bounds it, on one B200. 64 rows of 200 to 8192 tokens, 32 / 8 heads of 128 (163 MB of cache): 45 us. About 32 us
+// of them stream at 5 TB/s, 0.77 of the memory's measured rate, with issue slots 56 % and the ALU 51 % busy: four warps
+// per scheduler do not cover the latency of unpacking. The first data are there after 4.7 us; merging and stragglers
+// take 8. Two rows of 30 and 60 thousand tokens, 16 / 2 heads of 256 (52 MB): 29 us, 12 for the bytes, the rest the
+// merges of 37 CTAs per pair. One row of 2048 tokens (2.4 MB): 10 us, all of it latency.
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -37,11 +48,16 @@ using kv4::centre_odd;
 using kv4::Unit;
 using sm100::smem_u32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTree = 8;       // CTAs whose partials are merged first where a pair has more than kFlat
+// CTAs whose partials are merged first where a pair has more than kFlat: two rows over 37 CTAs per pair took 31.1 us
+// with 8, 32.0 with 6, 32.7 with 12.
+constexpr int kTree = 8;
 constexpr int kFlat = 24;
 constexpr int kMaxCtas = 32 * kTree;  // (a lane per partial)
-constexpr int kMinUnits = 3;   // units (and visits) of a warp below which fewer work
-constexpr int kVisit = 4;      // what a pair costs a warp besides its units, in units
+// Units (and visits) of a warp below which fewer CTAs work: one row of 2048 tokens took 12.6 us with 3, 14.6 with 8.
+constexpr int kMinUnits = 3;
+// What a pair costs a warp besides its units, in units: the 64 ragged rows above took 53.5 us with 0, 48.9 with 4, 47.3
+// with 8, 49.3 with 12.
+constexpr int kVisit = 8;
 constexpr float kHead = 7.f;   // log2 of how far a score may exceed the reference
 
 __device__ __forceinline__ float ex2(float x) {
@@ -88,21 +104,21 @@ struct DecodeArgs {
 
 constexpr int kMaxRows = 512;  // rows of one launch
 
-template <int HD, int NT>
+template <int HD>
 struct DecodeShape {
   // one CTA per SM (fewer partials to merge than several smaller ones), its warps by the registers:
   // 128 a thread, or 168
-  static constexpr int kWarps = NT == 1 && HD <= 128 ? 15 : 11;  // and one that issues the copies
+  static constexpr int kWarps = HD <= 128 ? 15 : 11;  // and one that issues the copies
   static constexpr int kThreads = (kWarps + 1) * 32;
   static_assert(2 * kWarps <= 32, "one lane per partial");
-  static constexpr int kStages = NT == 1 && HD <= 128 ? 3 : 4;                     // tiles in a warp's ring
+  static constexpr int kStages = HD <= 128 ? 3 : 4;                     // tiles in a warp's ring
   static constexpr int kTile = 256 / HD;                                           // units per stage (4608 bytes)
   static constexpr int kStageBytes = kTile * Unit<HD>::kBytes;
   static constexpr int kRow = HD + 4;  // floats of one head's partial: output, reference, sum
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kSmem = kWarps * kRing;  // the ring's place takes the part's last partial
   static_assert(kSmem + 10 * 1024 <= 227 * 1024, "shared memory of an SM");
-  static_assert(8 * NT * kRow * 4 <= kRing, "the last partial fits the ring");
+  static_assert(8 * kRow * 4 <= kRing, "the last partial fits the ring");
 };
 
 // A warp's partial in shared memory: units [u0, u1) of a pair.
@@ -190,11 +206,11 @@ __device__ __noinline__ void merge_parts(const float* from, bool live, int n, in
   }
 }
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
+template <int HD>
+__global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeArgs g_) {
   using U = Unit<HD>;
-  using Sh = DecodeShape<HD, NT>;
+  using Sh = DecodeShape<HD>;
   static_assert(kFlat <= 32 && kTree <= 32, "one lane per partial");
   constexpr int GR = HD / 64, KT = HD / 16, TU = Sh::kTile, kWarps = Sh::kWarps, kThreads = Sh::kThreads,
                 kStages = Sh::kStages;
@@ -263,8 +279,9 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     __syncthreads();
   }
   const int total = before[a.R];
-  // CTAs and warps at work: with few units every SM gets some before its warps multiply
-  const int W = min(kWarps, max(1, (total + (int)gridDim.x * kMinUnits - 1) / ((int)gridDim.x * kMinUnits)));
+  // CTAs and warps at work. A warp's part takes time, and so does each partial in its CTA's merge: with u units for a
+  // CTA, u / W + W is least at W = sqrt(u). (8 rows of 8000 tokens of two kv heads: 20.6 us, with sqrt(1.5 u) 22.8.)
+  const int W = min(kWarps, max(1, (int)ceilf(sqrtf((float)total / (float)gridDim.x))));
   const int N = min((int)gridDim.x, (total + W * kMinUnits - 1) / (W * kMinUnits));
   const int cta = blockIdx.x;
   // rows without context
@@ -407,75 +424,68 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     const int u_first = cc.u, h0 = head_of(cc.item), heads = heads_of(cc.item);
     const int len = rows[cc.row].y;
     // queries: B fragments (dims x 8 heads), float16 after a power-of-two scaling of each head
-    uint32_t qf[NT][KT][2];
-    float mult[NT][2], qsum[NT][2][GR];
+    uint32_t qf[KT][2];
+    float mult[2], qsum[2][GR];
+    uint4 raw[HD / 32];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      uint4 raw[HD / 32];
-      const int h = nt * 8 + fg;
+    for (int i = 0; i < HD / 32; ++i) {
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (fg < heads)
+        raw[i] = *reinterpret_cast<const uint4*>(a.q + cc.row * a.q_stride + (int64_t)(h0 + fg) * HD + 32 * i + 8 * ft);
+    }
+    __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (h < heads)
-          raw[i] = *reinterpret_cast<const uint4*>(a.q + cc.row * a.q_stride + (int64_t)(h0 + h) * HD + 32 * i + 8 * ft);
-      }
-      __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
+    for (int i = 0; i < HD / 32; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      for (int j = 0; j < 4; ++j) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
+    }
+    float mx = fmaxf(__low2float(top), __high2float(top));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // 2^-e with 1 <= mx 2^-e < 2 (1 for a zero, subnormal or non-finite head), exact in bf16
+    const int ex = (int)(__float_as_uint(mx) >> 23);
+    const bool norm = ex > 4 && ex < 254;
+    const uint32_t dn = norm ? (uint32_t)(254 - ex) << 7 : 0x3f80u, dn16 = dn + (4u << 7);
+    const uint32_t d1 = dn | dn << 16, d16 = dn16 | dn16 << 16;
+    // 2^24 of the subnormal codes, less the 16 of the query
+    const float un = norm ? __uint_as_float((uint32_t)ex << 23) : 1.f, up = un * (a.scale * kLog2e * 1048576.f);
+    float qs[GR];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
-      }
-      float mx = fmaxf(__low2float(top), __high2float(top));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // 2^-e with 1 <= mx 2^-e < 2 (1 for a zero, subnormal or non-finite head), exact in bf16
-      const int ex = (int)(__float_as_uint(mx) >> 23);
-      const bool norm = ex > 4 && ex < 254;
-      const uint32_t dn = norm ? (uint32_t)(254 - ex) << 7 : 0x3f80u, dn16 = dn + (4u << 7);
-      const uint32_t d1 = dn | dn << 16, d16 = dn16 | dn16 << 16;
-      // 2^24 of the subnormal codes, less the 16 of the query
-      const float un = norm ? __uint_as_float((uint32_t)ex << 23) : 1.f, up = un * (a.scale * kLog2e * 1048576.f);
-      float qs[GR];
+    for (int grp = 0; grp < GR; ++grp) qs[grp] = 0.f;
 #pragma unroll
-      for (int grp = 0; grp < GR; ++grp) qs[grp] = 0.f;
+    for (int i = 0; i < HD / 32; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // the odd nibbles' codes come 16 times larger
-          const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]),
-                                           *reinterpret_cast<const __nv_bfloat162*>(j & 1 ? &d1 : &d16));
-          const float lo = __low2float(y), hi = __high2float(y);
-          qf[nt][2 * i + j / 2][j & 1] = pack_f16(lo, hi);
-          qs[i / 2] = fmaf(lo + hi, j & 1 ? 1.f : 0.0625f, qs[i / 2]);
-        }
-      }
-#pragma unroll
-      for (int grp = 0; grp < GR; ++grp) {
-        qs[grp] += __shfl_xor_sync(0xffffffffu, qs[grp], 1);
-        qs[grp] += __shfl_xor_sync(0xffffffffu, qs[grp], 2);
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        mult[nt][c] = __shfl_sync(0xffffffffu, up, (2 * ft + c) * 4);
-#pragma unroll
-        for (int grp = 0; grp < GR; ++grp)
-          qsum[nt][c][grp] = __shfl_sync(0xffffffffu, qs[grp] * un, (2 * ft + c) * 4) * (a.scale * kLog2e);
+      for (int j = 0; j < 4; ++j) {  // the odd nibbles' codes come 16 times larger
+        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]),
+                                         *reinterpret_cast<const __nv_bfloat162*>(j & 1 ? &d1 : &d16));
+        const float lo = __low2float(y), hi = __high2float(y);
+        qf[2 * i + j / 2][j & 1] = pack_f16(lo, hi);
+        qs[i / 2] = fmaf(lo + hi, j & 1 ? 1.f : 0.0625f, qs[i / 2]);
       }
     }
-    float o[NT][KT][4], ref[NT][2], l[NT][2], oc[NT][2][GR];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int grp = 0; grp < GR; ++grp) {
+      qs[grp] += __shfl_xor_sync(0xffffffffu, qs[grp], 1);
+      qs[grp] += __shfl_xor_sync(0xffffffffu, qs[grp], 2);
+    }
 #pragma unroll
-      for (int m = 0; m < KT; ++m) o[nt][m][0] = o[nt][m][1] = o[nt][m][2] = o[nt][m][3] = 0.f;
+    for (int c = 0; c < 2; ++c) {
+      mult[c] = __shfl_sync(0xffffffffu, up, (2 * ft + c) * 4);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        ref[nt][c] = 0.f;
-        l[nt][c] = 0.f;
+      for (int grp = 0; grp < GR; ++grp)
+        qsum[c][grp] = __shfl_sync(0xffffffffu, qs[grp] * un, (2 * ft + c) * 4) * (a.scale * kLog2e);
+    }
+    float o[KT][4], ref[2], l[2], oc[2][GR];
 #pragma unroll
-        for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] = 0.f;
-      }
+    for (int m = 0; m < KT; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      ref[c] = 0.f;
+      l[c] = 0.f;
+#pragma unroll
+      for (int grp = 0; grp < GR; ++grp) oc[c][grp] = 0.f;
     }
     float log2_s = -24.f;  // E
     bool first = true;     // no reference yet
@@ -484,18 +494,16 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
       const int n = min(TU, u_last - cc.u);
       const uint8_t* base = ring + c_stage * Sh::kStageBytes;
       sm100::mbar_wait(&full[warp][c_stage], c_phase, a.status);
-      float s[TU][NT][4];
+      float s[TU][4];
       __half2 vp[TU][2][GR];
       // scores and value pairs of the tile
 #pragma unroll
       for (int j = 0; j < TU; ++j) {
         {
           const uint8_t* un = base + j * U::kBytes;
-          float acc[NT][GR][4];
+          float acc[GR][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int grp = 0; grp < GR; ++grp) acc[nt][grp][0] = acc[nt][grp][1] = acc[nt][grp][2] = acc[nt][grp][3] = 0.f;
+          for (int grp = 0; grp < GR; ++grp) acc[grp][0] = acc[grp][1] = acc[grp][2] = acc[grp][3] = 0.f;
 #pragma unroll
           for (int pl = 0; pl < (HD + 127) / 128; ++pl) {
             constexpr int W = HD < 128 ? 2 : 4;
@@ -514,35 +522,28 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
             for (int i = 0; i < W; ++i) {
               const int grp = pl * 2 + i / 2, k = pl * 8 + 2 * i;
               const uint32_t x = wa[i], y = wb[i], x8 = x >> 8, y8 = y >> 8;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_f16(acc[nt][grp], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[nt][k][0],
-                        qf[nt][k][1]);
-                mma_f16(acc[nt][grp], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
-                        qf[nt][k + 1][0], qf[nt][k + 1][1]);
-              }
+              mma_f16(acc[grp], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[k][0],
+                      qf[k][1]);
+              mma_f16(acc[grp], x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
+                      qf[k + 1][0], qf[k + 1][1]);
             }
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float x[NT][2], y[NT][2];
+            float x[2], y[2];
 #pragma unroll
             for (int grp = 0; grp < GR; ++grp) {
               vp[j][half][grp] = *reinterpret_cast<const __half2*>(un + U::pair(true, fg + 8 * half, grp));
               const float2 p = __half22float2(*reinterpret_cast<const __half2*>(un + U::pair(false, fg + 8 * half, grp)));
               const float b = fmaf(-8.f, p.x, p.y);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  x[nt][c] = grp ? fmaf(p.x, acc[nt][grp][2 * half + c], x[nt][c]) : p.x * acc[nt][grp][2 * half + c];
-                  y[nt][c] = fmaf(b, qsum[nt][c][grp], grp ? y[nt][c] : -ref[nt][c]);
-                }
+              for (int c = 0; c < 2; ++c) {
+                x[c] = grp ? fmaf(p.x, acc[grp][2 * half + c], x[c]) : p.x * acc[grp][2 * half + c];
+                y[c] = fmaf(b, qsum[c][grp], grp ? y[c] : -ref[c]);
+              }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) s[j][nt][2 * half + c] = fmaf(x[nt][c], mult[nt][c], y[nt][c]);
+            for (int c = 0; c < 2; ++c) s[j][2 * half + c] = fmaf(x[c], mult[c], y[c]);
           }
         }
       }
@@ -555,8 +556,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
             if ((cc.u + j) * 16 + fg + 8 * half >= lim) {
 #pragma unroll
               for (int grp = 0; grp < GR; ++grp) vp[j][half][grp] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) s[j][nt][2 * half] = s[j][nt][2 * half + 1] = -INFINITY;
+              s[j][2 * half] = s[j][2 * half + 1] = -INFINITY;
             }
       }
       // the tile's largest scale and scores: move the references where they are passed
@@ -573,43 +573,39 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
       }
       const float bound = kHead - log2_s;  // scores are relative to ref = R + E
       bool move = first || top_s > ex2(log2_s);
-      float mx[NT][2];
+      float mx[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int c = 0; c < 2; ++c) {
+        mx[c] = fmaxf(s[0][c], s[0][2 + c]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          mx[nt][c] = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
-#pragma unroll
-          for (int j = 1; j < TU; ++j) mx[nt][c] = fmaxf(mx[nt][c], fmaxf(s[j][nt][c], s[j][nt][2 + c]));
-          move |= mx[nt][c] > bound;
-        }
+        for (int j = 1; j < TU; ++j) mx[c] = fmaxf(mx[c], fmaxf(s[j][c], s[j][2 + c]));
+        move |= mx[c] > bound;
+      }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, off));
         // E: at least the exponent above the largest scale so far
         const float e_new = fmaxf(log2_s, (float)((int)(__float_as_uint(top_s) >> 23) - 126));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < 2; ++c) {
+          float m = mx[c];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m = mx[nt][c];
+          for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+          m += log2_s;  // the tile's largest score, relative to R
+          const float rise = m > -INFINITY && (first || m > 0.f) ? m : 0.f;
+          const float up_to = rise + (e_new - log2_s), corr = first ? 1.f : ex2(-up_to);
+          ref[c] += up_to;
+          l[c] *= corr;
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-            m += log2_s;  // the tile's largest score, relative to R
-            const float rise = m > -INFINITY && (first || m > 0.f) ? m : 0.f;
-            const float up_to = rise + (e_new - log2_s), corr = first ? 1.f : ex2(-up_to);
-            ref[nt][c] += up_to;
-            l[nt][c] *= corr;
+          for (int grp = 0; grp < GR; ++grp) oc[c][grp] *= corr;
 #pragma unroll
-            for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] *= corr;
-#pragma unroll
-            for (int k = 0; k < KT; ++k) {
-              o[nt][k][c] *= corr;
-              o[nt][k][2 + c] *= corr;
-            }
-#pragma unroll
-            for (int j = 0; j < TU; ++j) s[j][nt][c] -= up_to, s[j][nt][2 + c] -= up_to;
+          for (int k = 0; k < KT; ++k) {
+            o[k][c] *= corr;
+            o[k][2 + c] *= corr;
           }
+#pragma unroll
+          for (int j = 0; j < TU; ++j) s[j][c] -= up_to, s[j][2 + c] -= up_to;
+        }
         log2_s = e_new;
         first = false;
       }
@@ -617,7 +613,7 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
 #pragma unroll
       for (int j = 0; j < TU; ++j) {
         {
-          uint32_t pb[NT][GR][2];
+          uint32_t pb[GR][2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float sv[GR], vc[GR];
@@ -626,17 +622,14 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
               sv[grp] = __low2float(vp[j][half][grp]);
               vc[grp] = __high2float(vp[j][half][grp]);
             }
+            const float w0_ = ex2(s[j][2 * half]), w1_ = ex2(s[j][2 * half + 1]);
+            l[0] += w0_;
+            l[1] += w1_;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float w0_ = ex2(s[j][nt][2 * half]), w1_ = ex2(s[j][nt][2 * half + 1]);
-              l[nt][0] += w0_;
-              l[nt][1] += w1_;
-#pragma unroll
-              for (int grp = 0; grp < GR; ++grp) {
-                oc[nt][0][grp] = fmaf(w0_, vc[grp], oc[nt][0][grp]);
-                oc[nt][1][grp] = fmaf(w1_, vc[grp], oc[nt][1][grp]);
-                pb[nt][grp][half] = transpose8(pack_f16(w0_ * sv[grp], w1_ * sv[grp]));
-              }
+            for (int grp = 0; grp < GR; ++grp) {
+              oc[0][grp] = fmaf(w0_, vc[grp], oc[0][grp]);
+              oc[1][grp] = fmaf(w1_, vc[grp], oc[1][grp]);
+              pb[grp][half] = transpose8(pack_f16(w0_ * sv[grp], w1_ * sv[grp]));
             }
           }
           const uint8_t* vb = base + j * U::kBytes + U::kCodes + lane * 16;
@@ -649,11 +642,8 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
               const uint32_t lo = w[2 * il], hi = w[2 * il + 1], lo8 = lo >> 8, hi8 = hi >> 8;
               const uint32_t a0 = centre_even(lo), a1 = centre_odd(lo), a2 = centre_even(hi), a3 = centre_odd(hi);
               const uint32_t b0 = centre_even(lo8), b1 = centre_odd(lo8), b2 = centre_even(hi8), b3 = centre_odd(hi8);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_f16(o[nt][4 * grp + 2 * il], a0, a1, a2, a3, pb[nt][grp][0], pb[nt][grp][1]);
-                mma_f16(o[nt][4 * grp + 2 * il + 1], b0, b1, b2, b3, pb[nt][grp][0], pb[nt][grp][1]);
-              }
+              mma_f16(o[4 * grp + 2 * il], a0, a1, a2, a3, pb[grp][0], pb[grp][1]);
+              mma_f16(o[4 * grp + 2 * il + 1], b0, b1, b2, b3, pb[grp][0], pb[grp][1]);
             }
           }
         }
@@ -669,44 +659,42 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
     const int slot = cc.at + cc.units + kVisit >= p1 ? 1 : 0;  // the part's last pair: its ring is done
     float* mine = slot ? reinterpret_cast<float*>(ring) : firsts + warp * pstride;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int c = 0; c < 2; ++c) {
+      const int h = 2 * ft + c;
+      float lt = l[c], f = 1.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int h = nt * 8 + 2 * ft + c;
-        float lt = l[nt][c], f = 1.f;
+      for (int off = 4; off < 32; off <<= 1) {
+        lt += __shfl_xor_sync(0xffffffffu, lt, off);
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          lt += __shfl_xor_sync(0xffffffffu, lt, off);
-#pragma unroll
-          for (int grp = 0; grp < GR; ++grp) oc[nt][c][grp] += __shfl_xor_sync(0xffffffffu, oc[nt][c][grp], off);
+        for (int grp = 0; grp < GR; ++grp) oc[c][grp] += __shfl_xor_sync(0xffffffffu, oc[c][grp], off);
+      }
+      if (h < heads) {
+        float* to = mine + h * Sh::kRow + 4 * fg;  // fp32: the partial, or the output itself
+        uint16_t* to16 = nullptr;
+        if (whole) {
+          const int64_t at = (int64_t)(h0 + h) * HD + 4 * fg;
+          if (a.sinks) lt += ex2(fminf(a.sinks[h0 + h] * kLog2e - ref[c], 126.f));
+          f = __frcp_rn(lt);
+          to = a.out ? a.out + cc.row * a.outf_stride + at : nullptr;
+          to16 = a.out_bf16 ? a.out_bf16 + cc.row * a.out_stride + at : nullptr;
+        } else if (fg == 0) {
+          *reinterpret_cast<float2*>(mine + h * Sh::kRow + HD) = make_float2(ref[c], lt);
         }
-        if (h < heads) {
-          float* to = mine + h * Sh::kRow + 4 * fg;  // fp32: the partial, or the output itself
-          uint16_t* to16 = nullptr;
-          if (whole) {
-            const int64_t at = (int64_t)(h0 + h) * HD + 4 * fg;
-            if (a.sinks) lt += ex2(fminf(a.sinks[h0 + h] * kLog2e - ref[nt][c], 126.f));
-            f = __frcp_rn(lt);
-            to = a.out ? a.out + cc.row * a.outf_stride + at : nullptr;
-            to16 = a.out_bf16 ? a.out_bf16 + cc.row * a.out_stride + at : nullptr;
-          } else if (fg == 0) {
-            *reinterpret_cast<float2*>(mine + h * Sh::kRow + HD) = make_float2(ref[nt][c], lt);
-          }
 #pragma unroll
-          for (int k = 0; k < KT; k += 2) {
-            const int d = (k >> 2) * 64 + ((k >> 1) & 1) * 32;
-            const float z = oc[nt][c][k >> 2];
-            const float4 v = make_float4((o[nt][k][c] + z) * f, (o[nt][k][2 + c] + z) * f, (o[nt][k + 1][c] + z) * f,
-                                         (o[nt][k + 1][2 + c] + z) * f);
-            if (to) *reinterpret_cast<float4*>(to + d) = v;
-            if (to16) {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-              *reinterpret_cast<uint2*>(to16 + d) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-            }
+        for (int k = 0; k < KT; k += 2) {
+          const int d = (k >> 2) * 64 + ((k >> 1) & 1) * 32;
+          const float z = oc[c][k >> 2];
+          const float4 v = make_float4((o[k][c] + z) * f, (o[k][2 + c] + z) * f, (o[k + 1][c] + z) * f,
+                                       (o[k + 1][2 + c] + z) * f);
+          if (to) *reinterpret_cast<float4*>(to + d) = v;
+          if (to16) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+            *reinterpret_cast<uint2*>(to16 + d) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
           }
         }
       }
+    }
     if (!whole && lane == 0) parts[2 * warp + slot] = Part{cc.row, cc.item, u_first, cc.u};
     next_pair(cc);
   }
@@ -829,16 +817,16 @@ __global__ void __launch_bounds__(DecodeShape<HD, NT>::kThreads, 1)
   pdl_launch();
 }
 
-template <int HD, int NT>
+template <int HD>
 void launch_decode(const DecodeArgs& d, int sms, cudaStream_t s, bool pdl) {
-  using Sh = DecodeShape<HD, NT>;
+  using Sh = DecodeShape<HD>;
   static bool configured = false;  // per instantiation; one device per process
   if (!configured) {
-    HK_CUDA_CHECK(cudaFuncSetAttribute(kv4_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    HK_CUDA_CHECK(cudaFuncSetAttribute(kv4_decode_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Sh::kSmem));
     configured = true;
   }
-  launch(kv4_decode_kernel<HD, NT>, dim3(std::min(sms, kMaxCtas)), dim3(Sh::kThreads), Sh::kSmem, s, pdl, d);
+  launch(kv4_decode_kernel<HD>, dim3(std::min(sms, kMaxCtas)), dim3(Sh::kThreads), Sh::kSmem, s, pdl, d);
 }
 
 }  // namespace
@@ -860,14 +848,13 @@ void kv4_attention_decode_launch(const Kv4AttnArgs& args, const Kv4Workspace& ws
     if (d.a.out_bf16) d.a.out_bf16 += r0 * args.out_stride;
     d.part = ws.part;
     d.counters = ws.counters;
-    const bool wide = G > 8 && args.hd <= 128;  // two tiles of 8 heads share each key and value
-    d.heads_per_item = wide ? G : (G < 8 ? G : 8);
-    d.split = G > d.heads_per_item ? 1 : 0;
+    d.heads_per_item = G < 8 ? G : 8;
+    d.split = G > 8 ? 1 : 0;
     const int upb = args.block_size / 16;
     d.upb_shift = (upb & (upb - 1)) ? -1 : __builtin_ctz(upb);
-    if (args.hd == 64) wide ? launch_decode<64, 2>(d, ws.sms, s, pdl) : launch_decode<64, 1>(d, ws.sms, s, pdl);
-    else if (args.hd == 128) wide ? launch_decode<128, 2>(d, ws.sms, s, pdl) : launch_decode<128, 1>(d, ws.sms, s, pdl);
-    else if (args.hd == 256) launch_decode<256, 1>(d, ws.sms, s, pdl);
+    if (args.hd == 64) launch_decode<64>(d, ws.sms, s, pdl);
+    else if (args.hd == 128) launch_decode<128>(d, ws.sms, s, pdl);
+    else if (args.hd == 256) launch_decode<256>(d, ws.sms, s, pdl);
     else throw std::runtime_error("kv4 attention: head_dim 64, 128 or 256");
   }
 }

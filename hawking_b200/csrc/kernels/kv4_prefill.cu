@@ -21,6 +21,18 @@
 //
 // Rows of different sequences may share a CTA: it goes through their runs one after the other. Where there are
 // fewer CTAs than SMs the keys are split over blockIdx.z; the last CTA of a tile to arrive adds the parts.
+// One block of 512 threads per SM: the tiles fill the tensor memory (2 x 128 columns of scores, 2 x HD of output) and the
+// softmax threads need 168 registers, which the unpackers (112) and the issuing warpgroup (64) give up. Four unpacking
+// warps keep ahead of the products; with eight, in 640 threads, the softmax threads spilled and it was slower.
+//
+// What bounds it, on one B200, 32 / 8 heads of 128. 2048 rows after 6144 tokens: 302 us, 0.8 PFLOP/s, 0.49 of the
+// measured bf16 rate. 256 equal CTAs on 148 SMs take two turns where 1.73 would do; within a CTA 128 keys take 2.8 us,
+// the exchange of scores and weights through tensor memory 48 % busy and issue slots 47 %: the softmax of a tile, not
+// the products (1.8 us by themselves), paces the loop. A CTA's begin (queries read and scaled, first keys unpacked) takes 6.6 us and its
+// end (output read and written) 3.6, so 2048 rows from an empty cache, 8.5 tiles of keys on average, take 64 us.
+// Queries read and outputs written by 16 or 8 lanes per row instead of a thread per row cost more instructions than they
+// saved in lines: 70 us instead of 64. Fewer CTAs than SMs: 256 rows after 4096 tokens took 66 us with the keys split
+// over blockIdx.z and 102 without.
 // A value group that holds NaN is unpacked as zeros and noted: rows that see the token get NaN in its 64
 // dims at the end (a weight of zero times NaN would reach every row of the tile).
 #include <algorithm>
@@ -780,7 +792,8 @@ void kv4_attention_prefill_launch(const Kv4AttnArgs& args, const Kv4Workspace& w
   p.a = args;
   p.part = ws.part;
   p.counters = ws.counters;
-  // with fewer CTAs than SMs the keys are split over the rest
+  // with fewer CTAs than SMs the keys are split over the rest (256 rows after 4096 tokens: 66 us against 102; three short
+  // prompts of 64-wide heads, where there is little to split, 29.2 against 28.8)
   const int upb = args.block_size / 16;
   p.upb_shift = (upb & (upb - 1)) ? -1 : __builtin_ctz(upb);
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(32, ws.sms / (tiles * args.nkv)));

@@ -1,4 +1,4 @@
-"""Paged KV cache in 4 bits: Python surface of kv4_cache.cu and kv4_attention.cu.
+"""Paged KV cache in 4 bits: Python surface of kv4_cache.cu, kv4_decode.cu and kv4_prefill.cu.
 
 A layer's cache is uint8 ``[blocks, kv_heads, block_size / 16, 18 * head_dim]`` (``cache_shape``):
 16 tokens of one head per unit, a 4-bit code per value and one float16 pair (s, c) per token and 64

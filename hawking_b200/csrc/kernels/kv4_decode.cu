@@ -833,9 +833,9 @@ void launch_decode(const DecodeArgs& d, int sms, cudaStream_t s, bool pdl) {
 
 void kv4_attention_decode_launch(const Kv4AttnArgs& args, const Kv4Workspace& ws, cudaStream_t s, bool pdl) {
   const int G = args.nh / args.nkv;
-  // rows of a launch: the sum of their units x items stays below 2^31
-  const int64_t most = ((int64_t)args.max_blocks * (args.block_size / 16) + 1) * args.nkv * 2;
-  const int chunk = (int)std::min<int64_t>(kMaxRows, ((int64_t(1) << 31) - 1) / most);
+  // rows of a launch: the sum of their units and visits x items stays below 2^31 by more than the kernel adds to it
+  const int64_t most = ((int64_t)args.max_blocks * (args.block_size / 16) + kVisit) * args.nkv * 2;
+  const int chunk = (int)std::min<int64_t>(kMaxRows, ((int64_t(1) << 31) - (1 << 20)) / most);
   if (chunk < 1) throw std::runtime_error("kv4 attention decode: context x kv heads too large");
   for (int r0 = 0; r0 < args.R; r0 += chunk) {
     DecodeArgs d{};

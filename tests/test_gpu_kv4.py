@@ -156,6 +156,17 @@ def test_decode_row_counts(rows, ctx):
     _check(_run(kv4.attention_decode, *case), ref, tol, True)
 
 
+@pytest.mark.parametrize("rows,columns", [(600, 4), (40, 1 << 22)])
+def test_decode_in_several_launches(rows, columns):
+    """More rows than a launch holds, and a table so wide that a launch's work is bounded by what it could hold."""
+    q, cache, tab, row_seq, row_ctx = _attention_case(rows, 16, 8, 64, 16, [(i % 40, 1) for i in range(rows)])
+    wide = torch.full((tab.shape[0], columns), 1 << 30, dtype=torch.int32, device=DEV)
+    wide[:, :tab.shape[1]] = tab
+    case = (q, cache, wide, row_seq, row_ctx)
+    ref, tol = _attention64(*case, 1 / math.sqrt(64))
+    _check(_run(kv4.attention_decode, *case), ref, tol, True)
+
+
 @pytest.mark.parametrize("fn", [kv4.attention_decode, kv4.attention_prefill])
 def test_attention_empty_rows_and_sinks(fn):
     q, cache, tab, row_seq, row_ctx = _attention_case(3, 8, 2, 128, 32, [(70, 4), (0, 3), (200, 2)])

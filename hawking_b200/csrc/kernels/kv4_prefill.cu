@@ -12,6 +12,7 @@
 //                    writes the weights back over them and, at the end, the output
 //   warps 8-11       unpack 128 tokens at a time from global memory (registers one tile ahead) to two shared
 //                    memory stages of keys and of values
+//   warps 13-15      fetch the query rows by bulk copies at the begin
 //   warp 12          issues the matrix instructions: S_t = Q_t K^T (both operands in shared memory) and
 //                    O_t += P_t V (P from tensor memory), the two tiles alternating so that one tile's
 //                    products run during the other's softmax
@@ -25,13 +26,13 @@
 // softmax threads need 168 registers, which the unpackers (112) and the issuing warpgroup (64) give up. Four unpacking
 // warps keep ahead of the products; with eight, in 640 threads, the softmax threads spilled and it was slower.
 //
-// What bounds it, on one B200, 32 / 8 heads of 128. 2048 rows after 6144 tokens: 302 us, 0.8 PFLOP/s, 0.49 of the
+// What bounds it, on one B200, 32 / 8 heads of 128. 2048 rows after 6144 tokens: 301 us, 0.8 PFLOP/s, 0.49 of the
 // measured bf16 rate. 256 equal CTAs on 148 SMs take two turns where 1.73 would do; within a CTA 128 keys take 2.8 us,
 // the exchange of scores and weights through tensor memory 48 % busy and issue slots 47 %: the softmax of a tile, not
-// the products (1.8 us by themselves), paces the loop. A CTA's begin (queries read and scaled, first keys unpacked) takes 6.6 us and its
-// end (output read and written) 3.6, so 2048 rows from an empty cache, 8.5 tiles of keys on average, take 64 us.
-// Queries read and outputs written by 16 or 8 lanes per row instead of a thread per row cost more instructions than they
-// saved in lines: 70 us instead of 64. Fewer CTAs than SMs: 256 rows after 4096 tokens took 66 us with the keys split
+// the products (1.8 us by themselves), paces the loop. A CTA's begin (queries fetched and scaled, first keys unpacked) takes 6 us and its
+// end (output read and written) 3.6, so 2048 rows from an empty cache, 8.5 tiles of keys on average, take 59 us. Loads of
+// the query rows by a thread per row, 32 lines with every load, made that 64; 16 lanes per row with the maximum by
+// shuffles, and 8 lanes per row for the output, 70. Fewer CTAs than SMs: 256 rows after 4096 tokens took 66 us with the keys split
 // over blockIdx.z and 102 without.
 // A value group that holds NaN is unpacked as zeros and noted: rows that see the token get NaN in its 64
 // dims at the end (a weight of zero times NaN would reach every row of the tile).
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
   const Kv4AttnArgs& a = g_.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_ready[2], p_ready[2], o_done[2], q_ready;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_ready[2], p_ready[2], o_done[2], q_raw, q_ready;
   __shared__ uint32_t tmem_s;
   __shared__ int seq_s[kMaxRuns], ctx_s[kMaxRuns], run_at[kMaxRuns + 1], run_kv[kMaxRuns];
   __shared__ int nan_at[kMaxRuns][GR];  // first token of a run whose value group holds NaN
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
       mbar_init(&p_ready[i], 128);
       mbar_init(&o_done[i], 1);
     }
+    mbar_init(&q_raw, 1);
     mbar_init(&q_ready, 256);
     fence_barrier_init();
     kv_top_s = 0;
@@ -283,47 +285,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
       const int head = kvh * G + (m < m_end ? m % G : 0);
       const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t s_at = tmem + lane_at + t * 128, o_at = tmem + lane_at + 256 + t * 128;
+      // this thread's query row: float16 after an exact scaling, from the raw rows into the swizzled tile (both for all
+      // runs). The chunk that is read in step c, c ^ x i in GF(8), takes all banks in turn on both sides
+      float mult;
+      {
+        if (!mbar_wait(&q_raw, 0, nullptr)) {
+          set_error(a.status, HK_ERR_MBAR_TIMEOUT);
+          ok = false;
+        }
+        const int turn = ((i << 1) & 6) ^ (i & 4 ? 3 : 0);
+        uint4 qr[HD / 8];
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          qr[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (m < m_end) qr[c] = *reinterpret_cast<const uint4*>(smem + (t * 128 + i) * HD * 2 + 16 * (c ^ turn));
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");  // the tile lies where its raw rows did
+        __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
+        }
+        const float mx = fmaxf(__low2float(top), __high2float(top));
+        const int ex = (int)(__float_as_uint(mx) >> 23);
+        const bool norm = ex > 0 && ex < 254;  // 2^-e with 1 <= mx 2^-e < 2
+        const uint32_t dn = norm ? (uint32_t)(254 - ex) << 7 : 0x3f80u, dn2 = dn | dn << 16;
+        mult = (norm ? __uint_as_float((uint32_t)ex << 23) : 1.f) * (a.scale * kLog2e);
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&dn2));
+            w[k] = pack_f16(__low2float(y), __high2float(y));
+          }
+          const int chunk = c ^ turn;
+          *reinterpret_cast<uint4*>(smem + t * Sh::kQTile + (chunk >> 3) * Sh::kAtom + sw128_offset(i, chunk & 7)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+      }
       int s_phase = 0, o_phase = 0;
       for (int run = 0; run < n_runs && ok; ++run) {
         int t0, t1;
         tiles_of(run, t0, t1);
         const bool mine = my_row >= run_at[run] && my_row < run_at[run + 1];
         const int ctx = mine ? ctx_s[my_row] : 0;
-        float mult = 0.f, ref = -INFINITY, l = 0.f;
+        float ref = -INFINITY, l = 0.f;
         if (t1 > t0) {
-          // this thread's query row: float16 after an exact scaling, into the swizzled tile
-          const uint16_t* src = a.q + (int64_t)(row0 + max(my_row, 0)) * a.q_stride + (int64_t)head * HD;
-          uint4 qr[HD / 8];
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            qr[c] = make_uint4(0u, 0u, 0u, 0u);
-            if (mine) qr[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-          }
-          __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            const uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
-          }
-          const float mx = fmaxf(__low2float(top), __high2float(top));
-          const int ex = (int)(__float_as_uint(mx) >> 23);
-          const bool norm = ex > 0 && ex < 254;  // 2^-e with 1 <= mx 2^-e < 2
-          const uint32_t dn = norm ? (uint32_t)(254 - ex) << 7 : 0x3f80u, dn2 = dn | dn << 16;
-          mult = (norm ? __uint_as_float((uint32_t)ex << 23) : 1.f) * (a.scale * kLog2e);
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            uint32_t w[4] = {qr[c].x, qr[c].y, qr[c].z, qr[c].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]),
-                                               *reinterpret_cast<const __nv_bfloat162*>(&dn2));
-              w[k] = pack_f16(__low2float(y), __high2float(y));
-            }
-            *reinterpret_cast<uint4*>(smem + t * Sh::kQTile + (c >> 3) * Sh::kAtom + sw128_offset(i, c & 7)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          fence_proxy_async_smem();
           mbar_arrive(&q_ready);
           for (int j = t0; j < t1; ++j) {
             if (!(ok = mbar_wait(&s_ready[t], s_phase, a.status))) break;
@@ -698,6 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             if (more) ++n_k;
             p_phase ^= 1;
           }
+        }
+      } else {  // the query rows, as they lie, to the tiles' place: a row's heads of the kv head in one copy
+        if (tid == 13 * 32) mbar_arrive_expect_tx(&q_raw, (m_end - m0) * HD * 2);
+        for (int i = tid - 13 * 32; i < nrows; i += 3 * 32) {
+          const int b = max(m0, (row0 + i) * G), e = min(m_end, (row0 + i + 1) * G);
+          bulk_g2s(smem + (b - m0) * HD * 2,
+                   a.q + (int64_t)(row0 + i) * a.q_stride + (int64_t)(kvh * G + b - (row0 + i) * G) * HD, (e - b) * HD * 2,
+                   &q_raw);
         }
       }
     }

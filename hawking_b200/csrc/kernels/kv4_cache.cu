@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
         blk = a.tables[(int64_t)seq * a.max_blocks + col];
       }
       slot = blk < 0 ? -1 : blk * bs + pos % bs;
+      if (blk < 0) set_error(a.status, HK_ERR_BAD_ARG);  // the row's keys and values have no place
     }
     a.positions[r] = pos;
     a.row_seq[r] = seq;

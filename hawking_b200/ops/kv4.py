@@ -78,7 +78,8 @@ def plan_rows(seq_rows: torch.Tensor, cached: torch.Tensor, new: torch.Tensor, b
     number. Without it the tables must already hold them.
 
     A request that does not fit its table row (or has a negative length or a bad row) gets no rows;
-    rows that do not fit the outputs are dropped, rows whose block is missing get slot -1. Each sets
+    rows that do not fit the outputs are dropped, rows whose block is missing (a negative entry of the
+    table or the list, or a list too short) get slot -1. Each sets
     ``status`` to 4 (bad argument)."""
     launches.add()
     kernels().kv4_plan(seq_rows, cached, new, block_tables, block_size, positions, row_seq, row_ctx, slots,

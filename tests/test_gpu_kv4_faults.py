@@ -1,0 +1,40 @@
+"""The 4-bit KV cache's operators (ops/kv4.py) on what a caller can get wrong or a launch can fail at:
+rows without a place, numbers at the end of int32, inputs that a kernel must not be given."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from hawking_b200.ops import kv4  # noqa: E402
+
+DEV = "cuda"
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def _plan(seq, cached, new, tab, bs, cap, free=None):
+    """(rows, tables, blocks taken, status)."""
+    out = torch.full((4, cap), 77, dtype=torch.int32, device=DEV)
+    t, taken, status = _ints(tab) if isinstance(tab, list) else tab, _ints([-5]), _ints([0])
+    kv4.plan_rows(_ints(seq), _ints(cached), _ints(new), t, bs, *out.unbind(0),
+                  free_blocks=None if free is None else _ints(free), taken=taken, status=status)
+    torch.cuda.synchronize()
+    return out.t().tolist(), t, taken.item(), status.item()
+
+
+# ---- rows without a place ------------------------------------------------------------------------
+def test_plan_reports_rows_without_a_block():
+    """A negative table entry leaves a row without a slot: the step's status says so."""
+    for free in (None, [9, 8]):  # complete tables, and the partial block of a request that also takes new ones
+        tab = [[5, -1, 7], [4, 6, 0]]
+        rows, _, taken, status = _plan([0, 1], [30, 16], [2, 1], tab, 16, 3, free)
+        assert rows == [[30, 0, 31, -1], [31, 0, 32, -1], [16, 1, 17, 96 if free is None else 144]]
+        assert status == 4 and taken == (0 if free is None else 1)
+    rows, _, _, status = _plan([0], [15], [2], [[5, -1, 7]], 16, 2)
+    assert rows == [[15, 0, 16, 95], [16, 0, 17, -1]] and status == 4
+    rows, _, _, status = _plan([0], [16], [1], [[5, 0, 0]], 16, 1, [-3])  # a block list's entry
+    assert rows == [[16, 0, 17, -1]] and status == 4
+    # an entry that no live row looks up does not matter
+    assert _plan([0], [15], [1], [[5, -1, 7]], 16, 2)[3] == 0

@@ -95,8 +95,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
       } else {
         blk = a.tables[(int64_t)seq * a.max_blocks + col];
       }
-      slot = blk < 0 ? -1 : blk * bs + pos % bs;
-      if (blk < 0) set_error(a.status, HK_ERR_BAD_ARG);  // the row's keys and values have no place
+      // no block, or one whose slots no int32 holds: the row's keys and values have no place
+      const long long at = (long long)blk * bs + pos % bs;
+      if (blk >= 0 && at <= kTop) slot = (int)at;
+      else set_error(a.status, HK_ERR_BAD_ARG);
     }
     a.positions[r] = pos;
     a.row_seq[r] = seq;

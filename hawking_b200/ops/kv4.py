@@ -79,7 +79,7 @@ def plan_rows(seq_rows: torch.Tensor, cached: torch.Tensor, new: torch.Tensor, b
 
     A request that does not fit its table row (or has a negative length or a bad row) gets no rows;
     rows that do not fit the outputs are dropped, rows whose block is missing (a negative entry of the
-    table or the list, or a list too short) get slot -1. Each sets
+    table or the list, or a list too short) or too large for an int32 slot get slot -1. Each sets
     ``status`` to 4 (bad argument)."""
     launches.add()
     kernels().kv4_plan(seq_rows, cached, new, block_tables, block_size, positions, row_seq, row_ctx, slots,

@@ -38,3 +38,12 @@ def test_plan_reports_rows_without_a_block():
     assert rows == [[16, 0, 17, -1]] and status == 4
     # an entry that no live row looks up does not matter
     assert _plan([0], [15], [1], [[5, -1, 7]], 16, 2)[3] == 0
+
+
+def test_plan_reports_blocks_past_int32_slots():
+    """block * block_size past 2^31 is no slot (in 32 bits it would come out as another valid one)."""
+    for blk in (1 << 27, (1 << 28) + 3, 2 ** 31 - 1):
+        rows, _, _, status = _plan([0, 1], [0, 3], [1, 1], [[blk, 0], [6, 0]], 16, 2)
+        assert rows == [[0, 0, 1, -1], [3, 1, 4, 99]] and status == 4
+    rows, _, _, status = _plan([0], [0], [16], [[(1 << 27) - 1, 0]], 16, 16)  # the last block of all
+    assert status == 0 and [r[3] for r in rows] == list(range(2 ** 31 - 16, 2 ** 31))

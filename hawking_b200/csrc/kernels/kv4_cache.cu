@@ -18,6 +18,9 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanRows = 2048;    // rows per CTA
 constexpr int kPlanMaxSeqs = 8192;  // both scans in shared memory
 
+// blocks that n >= 0 tokens take (n may be near 2^31: no n + bs - 1)
+__device__ __forceinline__ int blocks_of(int n, int bs) { return n / bs + (n % bs != 0); }
+
 // index of the last entry of the non-decreasing a[0..n) that is <= v (a[0] == 0)
 __device__ __forceinline__ int last_not_above(const int* a, int n, int v) {
   int lo = 0, hi = n;
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
     const int c = a.cached[i], seq = a.seq_rows[i];
     // a request that cannot be laid out gets no rows
     if (n < 0 || c < 0 || seq < 0 || seq >= a.table_rows || (long long)c + n > room) n = 0, bad = true;
-    const int nd = n > 0 ? (c + n + bs - 1) / bs - (c + bs - 1) / bs : 0;
+    const int nd = n > 0 ? blocks_of(c + n, bs) - blocks_of(c, bs) : 0;
     start[i] = n;
     base[i] = nd;
     rows += n;
@@ -87,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
       seq = a.seq_rows[i];
       pos = c + r - start[i];
       ctx = pos + 1;
-      const int col = pos / bs, b0 = (c + bs - 1) / bs;
+      const int col = pos / bs, b0 = blocks_of(c, bs);
       int blk;
       if (take && col >= b0) {
         const long long j = (long long)base[i] + col - b0;
@@ -109,7 +112,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
     const int n = (int)min(total_need, (long long)a.n_free);
     for (int j = blockIdx.x * kPlanThreads + tid; j < n; j += gridDim.x * kPlanThreads) {
       const int i = last_not_above(base, a.S, j);
-      a.tables[(int64_t)a.seq_rows[i] * a.max_blocks + (a.cached[i] + bs - 1) / bs + j - base[i]] = a.free_blocks[j];
+      a.tables[(int64_t)a.seq_rows[i] * a.max_blocks + blocks_of(a.cached[i], bs) + j - base[i]] = a.free_blocks[j];
     }
   }
   if (blockIdx.x == 0 && tid == 0) {

@@ -47,3 +47,19 @@ def test_plan_reports_blocks_past_int32_slots():
         assert rows == [[0, 0, 1, -1], [3, 1, 4, 99]] and status == 4
     rows, _, _, status = _plan([0], [0], [16], [[(1 << 27) - 1, 0]], 16, 16)  # the last block of all
     assert status == 0 and [r[3] for r in rows] == list(range(2 ** 31 - 16, 2 ** 31))
+
+
+def test_plan_lengths_near_2_to_the_31():
+    """A table row whose last block ends just below 2^31 tokens: blocks are counted without passing int32."""
+    bs, width = 65535, 32768
+    tab = torch.full((3, width), 11, dtype=torch.int32, device=DEV)
+    last = (width - 1) * bs
+    rows, t, taken, status = _plan([2, 0, 1], [last, width * bs - 1, 0], [bs, 1, 1], tab.clone(), bs, bs + 2, [5, 4, 3])
+    assert status == 0 and taken == 2
+    assert rows[0] == [last, 2, last + 1, 5 * bs] and rows[bs - 1] == [last + bs - 1, 2, last + bs, 5 * bs + bs - 1]
+    assert rows[bs:] == [[width * bs - 1, 0, width * bs, 11 * bs + bs - 1], [0, 1, 1, 4 * bs]]
+    want = tab.clone()
+    want[2, -1], want[1, 0] = 5, 4
+    assert torch.equal(t, want)
+    # one token past the row's end gets no rows
+    assert _plan([0], [width * bs], [1], tab, bs, 1)[::3] == ([[0, 0, 0, -1]], 4)

@@ -183,7 +183,7 @@ void kv4_gather(const Tensor& cache, const Tensor& slots, const optional<Tensor>
 void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Tensor& block_tables,
                    const Tensor& row_seq, const Tensor& row_ctx, double scale, const optional<Tensor>& out,
                    const optional<Tensor>& out_bf16, const optional<Tensor>& sinks, const Tensor& status, const Tensor& part, const Tensor& counters,
-                   int64_t sms, bool pdl) {
+                   int64_t sms, bool pdl, int64_t wait_polls) {
   const Shape sh = cache_shape(cache);
   const at::Device dev = cache.device();
   TORCH_CHECK(q.device() == dev && q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == sh.hd &&
@@ -228,6 +228,9 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
     a.sinks = sinks->data_ptr<float>();
   }
   a.status = ints_out(status, 1, dev, "status");
+  TORCH_CHECK(wait_polls >= 0 && wait_polls <= hk::kKv4WaitPolls, "kv4 attention: wait_polls must be 0 to ",
+              num(hk::kKv4WaitPolls));
+  a.wait_polls = (uint32_t)wait_polls;
   TORCH_CHECK(part.device() == dev && part.scalar_type() == at::kFloat && part.is_contiguous() &&
                   part.numel() >= hk::kKv4PartFloats((int)sms) && sms > 0 && 3 * sms <= hk::kKv4Counters,
               "kv4 attention: the workspace's partials are too small");
@@ -256,7 +259,8 @@ void register_kv4_kernels(py::module_& m) {
   m.def("kv4_attention", &kv4_attention, py::arg("prefill"), py::arg("q"), py::arg("cache"), py::arg("block_tables"),
         py::arg("row_seq"), py::arg("row_ctx"), py::arg("scale"), py::arg("out"), py::arg("out_bf16"),
         py::arg("sinks"), py::arg("status"), py::arg("part"), py::arg("counters"), py::arg("sms"),
-        py::arg("pdl") = false);
+        py::arg("pdl") = false, py::arg("wait_polls") = (int64_t)hk::kKv4WaitPolls);
+  m.attr("KV4_WAIT_POLLS") = (int64_t)hk::kKv4WaitPolls;
   m.def("kv4_workspace_sizes", [](int64_t sms) { return std::make_pair(hk::kKv4PartFloats((int)sms), hk::kKv4Counters); });
 }
 }  // namespace hk

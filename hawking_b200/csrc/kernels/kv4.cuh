@@ -14,6 +14,7 @@
 #pragma once
 #include "common.cuh"
 #include "kv4.h"
+#include "sm100.cuh"
 
 namespace hk {
 namespace kv4 {
@@ -59,6 +60,33 @@ __device__ __forceinline__ uint32_t centre_odd(uint32_t w) {
 // Largest magnitude a group holds: larger finite values are clamped to it, so that the centre and
 // the ends c - 8 s, c + 7 s of every group stay finite in float16.
 constexpr float kMaxValue = 65024.f;
+
+// ---- waits of the attention kernels ----
+// A wait that ran out: over a bad argument's code, which is the lesser failure.
+__device__ __forceinline__ void timed_out(int* status) { atomicExch(status, HK_ERR_MBAR_TIMEOUT); }
+
+// A warp's bounded wait, with one answer for all lanes: those that give up leave the code in which a warp votes, or
+// issues instructions as one, together. It gives up after `polls` polls, or early once a wait anywhere has. (A bad
+// argument's code in the status word, of this launch or an earlier one, ends no wait: its rows read as zeros and the
+// other rows go on.)
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, uint32_t polls) {
+  bool done = false;
+  for (uint32_t i = 0; i < polls; ++i) {
+    if ((done = sm100::mbar_try_wait(bar, parity))) break;
+    if ((i & 1023) == 1023 && *reinterpret_cast<volatile int*>(status) == HK_ERR_MBAR_TIMEOUT) break;
+  }
+  done = __all_sync(0xffffffffu, done);
+  if (!done) timed_out(status);
+  return done;
+}
+
+// The wait for a CTA's own copies or products before it gives up its memory: whatever the status word says, and
+// however short the other waits are.
+__device__ __forceinline__ bool drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kKv4WaitPolls; ++i)
+    if (sm100::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
 
 }  // namespace kv4
 }  // namespace hk

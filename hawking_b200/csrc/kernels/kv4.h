@@ -65,7 +65,9 @@ struct Kv4AttnArgs {
   float* out;           // fp32, same shape and stride rule (outf_stride), or null
   int64_t out_stride, outf_stride;
   int* status;
+  uint32_t wait_polls;  // polls after which a wait gives up (HK_ERR_MBAR_TIMEOUT; the outputs are then undefined)
 };
+constexpr uint32_t kKv4WaitPolls = 1u << 22;  // a second or so; a wait takes microseconds
 
 // Scratch of the attention launches of one stream. counters are zero between launches.
 struct Kv4Workspace {

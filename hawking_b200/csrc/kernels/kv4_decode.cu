@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
   __shared__ int wsum[kWarps + 1];
   __shared__ Part parts[2 * kWarps];
   __shared__ int last_s[2];
+  __shared__ volatile int gave_up;       // a wait of this CTA ran out
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int fg = lane >> 2, ft = lane & 3;
   const int G = a.nh / a.nkv, items = a.nkv << g_.split, HPI = g_.heads_per_item;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
       if (lane >= o) inc += v;
     }
     if (lane == 31) wsum[warp] = inc;
-    if (tid == 0) before[0] = 0;
+    if (tid == 0) before[0] = gave_up = 0;
     __syncthreads();
     int base = inc - sum;
 #pragma unroll
@@ -335,6 +336,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
     }
   };
 
+  int c_stage = 0, c_phase = 0;  // next stage of the ring: to read, or (in the copying warp) to fill
   // ---- the copying warp: every lane fetches one warp's tiles, kStages ahead, so that the cursors and
   // addresses of all warps cost one warp's instructions ----
   if (copies) {
@@ -363,10 +365,11 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
     };
     uint8_t* const my_ring = smem + lane * Sh::kRing;
     int st = 0, ph = 1;
+    unsigned idle = 0;  // turns in a row in which no lane had a free stage (the same for the warp, as its ways out)
     bool more = lane < W && more_in(cc);
     if (more) lookup(true);
 #pragma unroll 1
-    for (unsigned spin = 0; __any_sync(0xffffffffu, more); ++spin) {
+    while (__any_sync(0xffffffffu, more)) {
       const bool go = more && sm100::mbar_try_wait(&empty[lane][st], ph);
       if (go) {
         const int n = min(TU, min(cc.units, p1 - cc.at) - cc.u);
@@ -403,24 +406,29 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
         if (pair) next_pair(cc);
         more = more_in(cc);
         if (more) lookup(pair);
-        spin = 0;
       }
-      if (!__any_sync(0xffffffffu, go)) {
-        if (spin > (1u << 24)) {  // warps that never free a stage
-          set_error(a.status, HK_ERR_MBAR_TIMEOUT);
+      if (__any_sync(0xffffffffu, go)) {
+        idle = 0;
+      } else {
+        const bool over = ++idle > a.wait_polls;  // warps that never free a stage
+        if (__any_sync(0xffffffffu, over || gave_up)) {
+          if (over) kv4::timed_out(a.status);
+          gave_up = 1;
           break;
         }
         __nanosleep(64);
       }
     }
+    c_stage = st;
+    c_phase = ph;
   }
 
   // ---- the other warps: one pair after the other. A pair's part goes out (if it is the whole pair) or to a
   // partial: the first of the warp's to global memory (its ring is in use), the last to the ring's place ----
   const int pstride = HPI * Sh::kRow;
   float* const firsts = g_.part + ((int64_t)gridDim.x * 2 + (int64_t)cta * kWarps) * pstride;
-  int c_stage = 0, c_phase = 0;
-  while (!copies && more_in(cc)) {
+  bool ok = true;  // the same for the warp
+  while (!copies && ok && more_in(cc)) {
     const int u_first = cc.u, h0 = head_of(cc.item), heads = heads_of(cc.item);
     const int len = rows[cc.row].y;
     // queries: B fragments (dims x 8 heads), float16 after a power-of-two scaling of each head
@@ -493,7 +501,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
     while (cc.u < u_last) {
       const int n = min(TU, u_last - cc.u);
       const uint8_t* base = ring + c_stage * Sh::kStageBytes;
-      sm100::mbar_wait(&full[warp][c_stage], c_phase, a.status);
+      if (!(ok = kv4::warp_wait(&full[warp][c_stage], c_phase, a.status, a.wait_polls))) break;
       float s[TU][4];
       __half2 vp[TU][2][GR];
       // scores and value pairs of the tile
@@ -654,6 +662,10 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
       if (++c_stage == kStages) c_stage = 0, c_phase ^= 1;
     }
 
+    if (!ok) {  // its stage is not freed: the copying warp ends too
+      gave_up = 1;
+      break;
+    }
     // ---- the pair's result in this part ----
     const bool whole = u_first == 0 && cc.u == cc.units;
     const int slot = cc.at + cc.units + kVisit >= p1 ? 1 : 0;  // the part's last pair: its ring is done
@@ -710,6 +722,11 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
   };
   // ---- pairs that span warps or CTAs (rolled loops: this code runs once per CTA, cold) ----
   __syncthreads();
+  if (gave_up) {  // nothing is merged; the CTA's memory stays until its copies have arrived
+    if (copies && lane < W)
+      for (int s = 0; s < kStages; ++s) kv4::drain(&full[lane][s], s < c_stage ? c_phase ^ 1 : c_phase);
+    return;
+  }
   // the CTA's pairs that reach into others: at most one at its begin (0) and one at its end (1)
   __shared__ int span[2][5];  // row (-1: none), item, CTAs c0 .. c1, slot of c0's partial (the others' are 0)
   if (tid < 2) span[tid][0] = -1;

@@ -47,7 +47,10 @@ def cache_shape(num_blocks: int, n_kv_heads: int, block_size: int, head_dim: int
 class Workspace:
     """What the attention launches of one stream share: the device status word, the partial results of
     rows that several CTAs work on, and their arrival counters (zero between launches). Use one
-    workspace per stream: launches that share one must be ordered."""
+    workspace per stream: launches that share one must be ordered.
+
+    ``wait_polls`` bounds the kernels' waits: one that runs out sets the status word to 3, leaves the
+    launch's outputs undefined and needs a ``reset`` before the next launch."""
 
     def __init__(self, device="cuda"):
         self.device = torch.device(device)
@@ -56,6 +59,7 @@ class Workspace:
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.part = torch.empty(floats, dtype=torch.float32, device=device)
         self.counters = torch.zeros(counters, dtype=torch.int32, device=device)
+        self.wait_polls = kernels().KV4_WAIT_POLLS
 
     def reset(self):
         """Clear the status word and the counters (after a launch reported a failed wait)."""
@@ -120,7 +124,7 @@ def attention_decode(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.T
     ``[rows, heads * head_dim]``. A row with no context gives zeros."""
     launches.add()
     kernels().kv4_attention(False, q, cache, block_tables, row_seq, row_ctx, scale, out, out_bf16, sinks, ws.status,
-                            ws.part, ws.counters, ws.sms, PDL)
+                            ws.part, ws.counters, ws.sms, PDL, ws.wait_polls)
 
 
 def attention_prefill(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, row_seq: torch.Tensor,
@@ -130,4 +134,4 @@ def attention_prefill(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.
     ``row_ctx``; head_dim 64 or 128."""
     launches.add()
     kernels().kv4_attention(True, q, cache, block_tables, row_seq, row_ctx, scale, out, out_bf16, sinks, ws.status,
-                            ws.part, ws.counters, ws.sms, PDL)
+                            ws.part, ws.counters, ws.sms, PDL, ws.wait_polls)

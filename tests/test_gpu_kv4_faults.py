@@ -63,3 +63,68 @@ def test_plan_lengths_near_2_to_the_31():
     assert torch.equal(t, want)
     # one token past the row's end gets no rows
     assert _plan([0], [width * bs], [1], tab, bs, 1)[::3] == ([[0, 0, 0, -1]], 4)
+
+
+# ---- waits ---------------------------------------------------------------------------------------
+def _attention(hd, spans, nh=8, nkv=2, bs=32):
+    """(q, cache, tables, row_seq, row_ctx): random codes; spans lists (context before, rows) of each sequence."""
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    need = [-(-(a + n) // bs) for a, n in spans]
+    cache = torch.randint(0, 256, kv4.cache_shape(sum(need), nkv, bs, hd), dtype=torch.uint8, device=DEV, generator=g)
+    pairs = torch.rand(*cache.shape[:3], 64 * (hd // 64), device=DEV, generator=g) * 0.2 + 0.05
+    cache[..., 16 * hd:] = pairs.half().view(torch.uint8)
+    tab, at = torch.zeros(len(spans), max(need), dtype=torch.int32, device=DEV), 0
+    for i, m in enumerate(need):
+        tab[i, :m] = torch.arange(at, at + m, device=DEV)
+        at += m
+    row_seq = _ints([i for i, (_, n) in enumerate(spans) for _ in range(n)])
+    row_ctx = _ints([a + j + 1 for a, n in spans for j in range(n)])
+    q = torch.randn(len(row_seq), nh, hd, device=DEV, generator=g).bfloat16()
+    return q, cache, tab, row_seq, row_ctx
+
+
+WAITING = [(kv4.attention_decode, 64, [(9000, 1), (3, 1), (700, 1)]), (kv4.attention_decode, 128, [(300, 20), (40000, 2)]),
+           (kv4.attention_decode, 256, [(20000, 1), (500, 1)])]
+
+
+def _attend(fn, case, ws):
+    out = torch.full((case[0].shape[0], 8 * case[0].shape[2]), 7.0, dtype=torch.bfloat16, device=DEV)
+    fn(*case, 0.1, ws, out_bf16=out)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("fn,hd,spans", WAITING)
+def test_a_bad_arguments_code_ends_no_wait(fn, hd, spans):
+    """The status word holds a bad argument's code, of an earlier launch or of this one's other rows: a row's
+    result is what it is without."""
+    q, cache, tab, row_seq, row_ctx = case = _attention(hd, spans)
+    ws = kv4.Workspace(DEV)
+    want = _attend(fn, case, ws)
+    assert ws.status.item() == 0
+    ws.status.fill_(4)
+    for _ in range(5):
+        assert torch.equal(_attend(fn, case, ws), want) and ws.status.item() == 4
+    ws.status.zero_()
+    bad = row_seq.clone()
+    bad[-1] = 77
+    for _ in range(5):
+        assert torch.equal(_attend(fn, (q, cache, tab, bad, row_ctx), ws)[:-1], want[:-1]) and ws.status.item() == 4
+
+
+@pytest.mark.parametrize("fn,hd,spans", WAITING)
+def test_a_wait_that_runs_out_ends_the_launch(fn, hd, spans):
+    """Every wait gives up at once, or after a few polls: the launch returns with the timeout's code, over that of a bad
+    argument, and after a reset the workspace works as before."""
+    case = _attention(hd, spans)
+    ws = kv4.Workspace(DEV)
+    want = _attend(fn, case, ws)
+    polls = ws.wait_polls
+    for n, before in ((0, 0), (0, 4), (1, 0), (2, 0), (5, 0), (20, 0)):
+        ws.wait_polls = n
+        ws.status.fill_(before)
+        _attend(fn, case, ws)
+        assert ws.status.item() == 3 if n == 0 else ws.status.item() in (0, 3)
+        ws.reset()
+        ws.wait_polls = polls
+        assert torch.equal(_attend(fn, case, ws), want) and ws.status.item() == 0

@@ -71,10 +71,8 @@ __device__ __forceinline__ void timed_out(int* status) { atomicExch(status, HK_E
 // other rows go on.)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, uint32_t polls) {
   bool done = false;
-  for (uint32_t i = 0; i < polls; ++i) {
-    if ((done = sm100::mbar_try_wait(bar, parity))) break;
-    if ((i & 1023) == 1023 && *reinterpret_cast<volatile int*>(status) == HK_ERR_MBAR_TIMEOUT) break;
-  }
+  for (uint32_t left = polls; left && !(done = sm100::mbar_try_wait(bar, parity)); --left)
+    if ((left & 1023) == 1 && *reinterpret_cast<volatile int*>(status) == HK_ERR_MBAR_TIMEOUT) break;
   done = __all_sync(0xffffffffu, done);
   if (!done) timed_out(status);
   return done;

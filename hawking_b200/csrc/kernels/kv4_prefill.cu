@@ -197,11 +197,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
   const Kv4AttnArgs& a = g_.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_ready[2], p_ready[2], o_done[2], q_raw, q_ready;
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_ready[2], p_ready[2], o_done[2], q_raw, q_ready, ended;
   __shared__ uint32_t tmem_s;
   __shared__ int seq_s[kMaxRuns], ctx_s[kMaxRuns], run_at[kMaxRuns + 1], run_kv[kMaxRuns];
   __shared__ int nan_at[kMaxRuns][GR];  // first token of a run whose value group holds NaN
   __shared__ int n_runs_s, kv_top_s, last_s;
+  __shared__ volatile int gave_up;      // a wait of this CTA ran out
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wg = tid >> 7;
   const int G = a.nh / a.nkv, kvh = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y;  // longest rows first
   const int m0 = tile * kRows, m_end = min(m0 + kRows, a.R * G);  // flat (row, head) pairs
@@ -219,8 +220,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     }
     mbar_init(&q_raw, 1);
     mbar_init(&q_ready, 256);
+    mbar_init(&ended, 1);
     fence_barrier_init();
-    kv_top_s = 0;
+    kv_top_s = gave_up = 0;
   }
   pdl_wait();
   if (warp == 12) {  // (not before: a CTA of the previous launch may still need its columns to finish)
@@ -274,7 +276,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     t0 = n * z / Z;
     t1 = n * (z + 1) / Z;
   };
-  bool ok = true;
+  bool ok = true;  // the same for a warp
+  const auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return ok = kv4::warp_wait(bar, parity, a.status, a.wait_polls);
+  };
   const uint32_t smem_q = smem_u32(smem), smem_k = smem_q + Sh::kOffK, smem_v = smem_q + Sh::kOffV;
   if (z < Z) {
     if (wg < 2) {
@@ -289,9 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
       // runs). The chunk that is read in step c, c ^ x i in GF(8), takes all banks in turn on both sides
       float mult;
       {
-        if (!mbar_wait(&q_raw, 0, nullptr)) {
-          set_error(a.status, HK_ERR_MBAR_TIMEOUT);
-          ok = false;
+        if (!(ok = __all_sync(0xffffffffu, kv4::drain(&q_raw, 0)))) {  // (the CTA's memory stays until they have arrived)
+          kv4::timed_out(a.status);
         }
         const int turn = ((i << 1) & 6) ^ (i & 4 ? 3 : 0);
         uint4 qr[HD / 8];
@@ -338,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         if (t1 > t0) {
           mbar_arrive(&q_ready);
           for (int j = t0; j < t1; ++j) {
-            if (!(ok = mbar_wait(&s_ready[t], s_phase, a.status))) break;
+            if (!wait(&s_ready[t], s_phase)) break;
             s_phase ^= 1;
             tc_fence_after();
             const int left = ctx - j * kKeys;  // tokens of the tile that the row sees
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             tc_fence_before();
             mbar_arrive(&p_ready[t]);
           }
-          if (ok && (ok = mbar_wait(&o_done[t], o_phase, a.status))) {
+          if (ok && wait(&o_done[t], o_phase)) {
             o_phase ^= 1;
             tc_fence_after();
           }
@@ -433,6 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
+          __syncwarp();  // (rows that are not of this run skip the rest of the turn)
           if (any) {  // (the same for the whole warp)
             tmem_ld_x32(o_at + c, o);
             tmem_wait_ld();
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
           int blk0 = block_of(u + 8), blk1 = block_of(u + 9);  // of the tile after the loaded one
           for (int j = t0; j < t1; ++j, ++n_done) {
             const int st = n_done & 1;
-            if (!(ok = mbar_wait(&k_empty[st], ((n_done >> 1) & 1) ^ 1, a.status))) break;
+            if (!wait(&k_empty[st], ((n_done >> 1) & 1) ^ 1)) break;
             const uint32_t ks = smem_k + st * Sh::kKStage + (32 * w + (kx >> 1) * 8 + b * 4 + (kx & 1)) * 128;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -613,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     c2[x][h][g] = cv & keep;
                   }
             }
-            if (!(ok = mbar_wait(&v_empty[st], ((n_done >> 1) & 1) ^ 1, a.status))) break;
+            if (!wait(&v_empty[st], ((n_done >> 1) & 1) ^ 1)) break;
             const uint32_t vs = smem_v + st * Sh::kVStage + (w >> 1) * HD * 128 + 4 * vg * 128;
 #pragma unroll
             for (int g = 0; g < GR; ++g)
@@ -683,8 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
           int t0, t1;
           tiles_of(run, t0, t1);
           if (t1 <= t0) continue;
-          ok = mbar_wait(&q_ready, q_phase, a.status) && mbar_wait(&k_full[n_k & 1], (n_k >> 1) & 1, a.status);
-          if (!ok) break;
+          if (!wait(&q_ready, q_phase) || !wait(&k_full[n_k & 1], (n_k >> 1) & 1)) break;
           q_phase ^= 1;
           tc_fence_after();
           scores(0, n_k & 1);
@@ -694,11 +698,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
           for (int j = t0; j < t1 && ok; ++j, ++n_v) {
             const int vst = n_v & 1, kst = n_k & 1;
             const bool more = j + 1 < t1;
-            ok = mbar_wait(&v_full[vst], (n_v >> 1) & 1, a.status);
+            wait(&v_full[vst], (n_v >> 1) & 1);
 #pragma unroll 1
             for (int t = 0; t < 2; ++t) {
-              if (ok) ok = mbar_wait(&p_ready[t], p_phase, a.status);
-              if (ok && more && t == 0) ok = mbar_wait(&k_full[kst], (n_k >> 1) & 1, a.status);
+              if (ok) wait(&p_ready[t], p_phase);
+              if (ok && more && t == 0) wait(&k_full[kst], (n_k >> 1) & 1);
               if (!ok) break;
               tc_fence_after();
               output(t, vst, j > t0);
@@ -721,14 +725,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         }
       }
     }
+    if (!ok) gave_up = 1;
   }
   __syncthreads();
   tc_fence_after();
   if (warp == 12) {
     __syncwarp();
+    if (gave_up) {  // products may be under way
+      commit_elected(&ended);
+      kv4::drain(&ended, 0);
+      __syncwarp();
+    }
     tmem_dealloc(tmem, 512);
   }
-  if (z >= Z || Z == 1) return;
+  if (z >= Z || Z == 1 || gave_up) return;
   // ---- parts of the keys: the last CTA of the tile adds them, in order ----
   __threadfence();
   __syncthreads();

@@ -84,7 +84,8 @@ def _attention(hd, spans, nh=8, nkv=2, bs=32):
 
 
 WAITING = [(kv4.attention_decode, 64, [(9000, 1), (3, 1), (700, 1)]), (kv4.attention_decode, 128, [(300, 20), (40000, 2)]),
-           (kv4.attention_decode, 256, [(20000, 1), (500, 1)])]
+           (kv4.attention_decode, 256, [(20000, 1), (500, 1)]), (kv4.attention_prefill, 64, [(5000, 300), (0, 70)]),
+           (kv4.attention_prefill, 128, [(6000, 40)]), (kv4.attention_prefill, 128, [(0, 3000), (100, 1000)])]
 
 
 def _attend(fn, case, ws):

@@ -136,8 +136,8 @@ void kv4_append(const Tensor& qkv, const Tensor& positions, const optional<Tenso
   TORCH_CHECK(rot_dim >= 0 && rot_dim % 2 == 0 && rot_dim <= hd, "kv4 append: rot_dim must be even and at most head_dim");
   TORCH_CHECK(style == 0 || style == 1, "kv4 append: style 0 (adjacent pairs) or 1 (halves)");
   TORCH_CHECK(rope.device() == dev && rope.scalar_type() == at::kFloat && rope.is_contiguous() && rope.dim() == 3 &&
-                  rope.size(1) * 2 == rot_dim && rope.size(2) == 2,
-              "kv4 append: rope must be contiguous fp32 [positions, rot_dim / 2, 2]");
+                  rope.size(1) * 2 == rot_dim && rope.size(2) == 2 && reinterpret_cast<uintptr_t>(rope.data_ptr()) % 8 == 0,
+              "kv4 append: rope must be 8-byte aligned contiguous fp32 [positions, rot_dim / 2, 2]");
   a.rope = rope.data_ptr<float>();
   a.rope_rows = (int)rope.size(0);
   a.rot_dim = (int)rot_dim;

@@ -129,3 +129,24 @@ def test_a_wait_that_runs_out_ends_the_launch(fn, hd, spans):
         ws.reset()
         ws.wait_polls = polls
         assert torch.equal(_attend(fn, case, ws), want) and ws.status.item() == 0
+
+
+# ---- inputs that a kernel must not be given ------------------------------------------------------
+def _append_args(R=2, nh=8, nkv=2, hd=64, bs=16):
+    return dict(qkv=torch.randn(R, (nh + 2 * nkv) * hd, device=DEV), pos=_ints(list(range(R))), slots=_ints(list(range(R))),
+                rope=torch.randn(R, hd // 2, 2, device=DEV), rot=hd, style=0,
+                q=torch.empty(R, nh, hd, dtype=torch.bfloat16, device=DEV),
+                cache=torch.zeros(kv4.cache_shape(2, nkv, bs, hd), dtype=torch.uint8, device=DEV), nh=nh, nkv=nkv, hd=hd)
+
+
+def test_append_refuses_a_rotation_table_off_its_boundary():
+    """(cos, sin) pairs are read as 8 bytes."""
+    a = _append_args()
+    n = a["rope"].numel()
+    shifted = torch.zeros(n + 2, device=DEV)
+    a["rope"] = shifted[1:n + 1].view(2, 32, 2)
+    with pytest.raises(RuntimeError, match="8-byte aligned"):
+        kv4.rope_append(*a.values())
+    a["rope"] = shifted[2:].view(2, 32, 2)
+    kv4.rope_append(*a.values())
+    torch.cuda.synchronize()

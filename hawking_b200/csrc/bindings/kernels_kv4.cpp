@@ -44,6 +44,7 @@ Shape cache_shape(const Tensor& c) {
   const int64_t hd = c.size(3) / 18;
   TORCH_CHECK(c.size(3) % 18 == 0 && (hd == 64 || hd == 128 || hd == 256),
               "kv4: head_dim must be 64, 128 or 256 (units of 18 * head_dim bytes), not units of ", num(c.size(3)), " bytes");
+  TORCH_CHECK(c.size(1) > 0 && c.size(2) > 0, "kv4: the cache must have kv heads and a block size of at least 16");
   TORCH_CHECK(aligned16(c.data_ptr()), "kv4: the cache must start on a 16-byte boundary");
   TORCH_CHECK(c.size(0) * c.size(2) * 16 < (int64_t(1) << 31), "kv4: KV pool too large for int32 slot ids");
   return {c.size(0), (int)c.size(1), (int)hd, (int)c.size(2) * 16};

@@ -150,3 +150,25 @@ def test_append_refuses_a_rotation_table_off_its_boundary():
     a["rope"] = shifted[2:].view(2, 32, 2)
     kv4.rope_append(*a.values())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 1), (2, 2, 0), (0, 0, 0)])
+def test_a_cache_without_heads_or_tokens_is_refused(shape):
+    """The host divides by the kv heads, the kernels by the block size."""
+    cache = torch.zeros(*shape, 18 * 64, dtype=torch.uint8, device=DEV)
+    ws, one = kv4.Workspace(DEV), _ints([0])
+    q, out = (torch.zeros(*s, dtype=torch.bfloat16, device=DEV) for s in ((1, 4, 64), (1, 256)))
+    for fn in (kv4.attention_decode, kv4.attention_prefill):
+        with pytest.raises(RuntimeError, match="kv heads and a block size"):
+            fn(q, cache, _ints([[0]]), one, one, 0.1, ws, out_bf16=out)
+    with pytest.raises(RuntimeError, match="kv heads and a block size"):
+        kv4.gather(cache, one, torch.zeros(1, shape[1], 64, dtype=torch.bfloat16, device=DEV), None)
+    a = _append_args(R=1)
+    a["cache"] = cache
+    with pytest.raises(RuntimeError, match="kv heads and a block size"):
+        kv4.rope_append(*a.values())
+    # blocks alone may be none: every slot is past such a cache
+    none = torch.zeros(kv4.cache_shape(0, 2, 16, 64), dtype=torch.uint8, device=DEV)
+    k = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    kv4.gather(none, one, k, None)
+    assert (k == 0).all()

@@ -145,8 +145,8 @@ void kv4_append(const Tensor& qkv, const Tensor& positions, const optional<Tenso
   a.rope_style = (int)style;
   TORCH_CHECK(q_out.device() == dev && q_out.scalar_type() == at::kBFloat16 && q_out.dim() == 3 && q_out.size(0) == a.R &&
                   q_out.size(1) == nh && q_out.size(2) == hd && q_out.stride(2) == 1 && q_out.stride(1) == hd &&
-                  q_out.stride(0) % 8 == 0 && aligned16(q_out.data_ptr()),
-              "kv4 append: q_out must be 16-byte aligned bf16 [rows, heads, head_dim]");
+                  (a.R < 2 || (q_out.stride(0) % 8 == 0 && q_out.stride(0) >= nh * hd)) && aligned16(q_out.data_ptr()),
+              "kv4 append: q_out must be 16-byte aligned bf16 [rows, heads, head_dim], no rows over one another");
   a.q_out = ptr<uint16_t>(q_out);
   a.q_stride = q_out.stride(0);
   a.cache = ptr<uint8_t>(cache);
@@ -215,8 +215,8 @@ void kv4_attention(bool prefill, const Tensor& q, const Tensor& cache, const Ten
     if (!t.has_value()) return nullptr;
     TORCH_CHECK(t->device() == dev && t->scalar_type() == ty && t->dim() == 2 && t->size(0) == a.R &&
                     t->size(1) == (int64_t)a.nh * a.hd && t->stride(1) == 1 &&
-                    (a.R < 2 || t->stride(0) % 8 == 0) && aligned16(t->data_ptr()),
-                "kv4 attention: ", name, " must be 16-byte aligned [rows, heads * head_dim]");
+                    (a.R < 2 || (t->stride(0) % 8 == 0 && t->stride(0) >= t->size(1))) && aligned16(t->data_ptr()),
+                "kv4 attention: ", name, " must be 16-byte aligned [rows, heads * head_dim], no rows over one another");
     stride = t->stride(0);
     return t->data_ptr();
   };

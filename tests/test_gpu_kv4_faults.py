@@ -172,3 +172,19 @@ def test_a_cache_without_heads_or_tokens_is_refused(shape):
     k = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
     kv4.gather(none, one, k, None)
     assert (k == 0).all()
+
+
+def test_outputs_whose_rows_lie_over_one_another_are_refused():
+    q, cache, tab, row_seq, row_ctx = _attention(64, [(5, 3)])
+    ws = kv4.Workspace(DEV)
+    for fn in (kv4.attention_decode, kv4.attention_prefill):
+        for dtype, name in ((torch.bfloat16, "out_bf16"), (torch.float32, "out")):
+            one = torch.zeros(1, 512, dtype=dtype, device=DEV)
+            with pytest.raises(RuntimeError, match="over one another"):
+                fn(q, cache, tab, row_seq, row_ctx, 0.1, ws, **{name: one.expand(3, 512)})
+            with pytest.raises(RuntimeError, match="over one another"):
+                fn(q, cache, tab, row_seq, row_ctx, 0.1, ws, **{name: one.new_zeros(2048).as_strided((3, 512), (504, 1))})
+    a = _append_args()
+    a["q"] = a["q"][:1].expand(2, 8, 64)
+    with pytest.raises(RuntimeError, match="over one another"):
+        kv4.rope_append(*a.values())

@@ -61,6 +61,18 @@ __device__ __forceinline__ uint32_t centre_odd(uint32_t w) {
 // the ends c - 8 s, c + 7 s of every group stay finite in float16.
 constexpr float kMaxValue = 65024.f;
 
+// ---- sinks of the attention kernels ----
+// A head's extra logit as log2 of its weight: NaN stays, and +infinity becomes a number that no score reaches, so that it
+// takes all the weight and no difference of infinities arises, whether a row is merged from parts or not.
+__device__ __forceinline__ float min_keeping_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float sink_log2(float sink) { return min_keeping_nan(sink * 1.4426950408889634f, 1e30f); }
+// log2 of its weight relative to a row's reference, of which the power stays finite
+__device__ __forceinline__ float sink_over(float sink, float ref) { return min_keeping_nan(sink_log2(sink) - ref, 126.f); }
+
 // ---- waits of the attention kernels ----
 // A wait that ran out: over a bad argument's code, which is the lesser failure.
 __device__ __forceinline__ void timed_out(int* status) { atomicExch(status, HK_ERR_MBAR_TIMEOUT); }

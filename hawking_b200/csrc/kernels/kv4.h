@@ -60,7 +60,7 @@ struct Kv4AttnArgs {
   const int *row_seq, *row_ctx;
   float scale;
   int R, nh, nkv, hd, block_size;
-  const float* sinks;   // [nh] extra logit per head, or null
+  const float* sinks;   // [nh] extra logit per head, or null (NaN: the head is NaN; +infinity: it is zero)
   uint16_t* out_bf16;   // [R, nh * hd] with row stride out_stride, or null
   float* out;           // fp32, same shape and stride rule (outf_stride), or null
   int64_t out_stride, outf_stride;

@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
         uint16_t* to16 = nullptr;
         if (whole) {
           const int64_t at = (int64_t)(h0 + h) * HD + 4 * fg;
-          if (a.sinks) lt += ex2(fminf(a.sinks[h0 + h] * kLog2e - ref[c], 126.f));
+          if (a.sinks) lt += ex2(kv4::sink_over(a.sinks[h0 + h], ref[c]));
           f = __frcp_rn(lt);
           to = a.out ? a.out + cc.row * a.outf_stride + at : nullptr;
           to16 = a.out_bf16 ? a.out_bf16 + cc.row * a.out_stride + at : nullptr;
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(DecodeShape<HD>::kThreads, 1)
   }
 
   const auto sink_of = [&](const float* dst, int item, int h) {
-    return !dst && a.sinks ? a.sinks[head_of(item) + h] * kLog2e : -INFINITY;
+    return !dst && a.sinks ? kv4::sink_log2(a.sinks[head_of(item) + h]) : -INFINITY;
   };
   const auto merge_to = [&](float* dst, int row, int item, int h, int ml_at) {
     const int64_t at = (int64_t)(head_of(item) + h) * HD;

@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         float f = 0.f;
         if (Z == 1 && any) {
           float lt = l;
-          if (a.sinks) lt += ex2(fminf(a.sinks[head] * kLog2e - (ref > -INFINITY ? ref : 0.f), 126.f));
+          if (a.sinks) lt += ex2(kv4::sink_over(a.sinks[head], ref > -INFINITY ? ref : 0.f));
           f = ctx > 0 ? __frcp_rn(lt) : 0.f;
         } else if (any) {
           f = 1.f;
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int i = x / (HD / 4), d = x % (HD / 4) * 4, m = m0 + i;
     const int row = m / G, head = kvh * G + m % G;
     const float* p = first + (int64_t)i * (HD + 4);
-    float r = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
+    float r = a.sinks ? kv4::sink_log2(a.sinks[head]) : -INFINITY;
     float lt = a.sinks ? 1.f : 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = 0; k0 < Z; k0 += 4) {

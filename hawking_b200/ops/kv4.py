@@ -121,7 +121,8 @@ def attention_decode(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.T
     """Attention of bf16 queries ``[rows, heads, head_dim]`` over the first ``row_ctx`` cached tokens
     of each row's sequence, for rows that are one token of a sequence each (any mix is right, long
     runs of one sequence are faster in ``attention_prefill``). ``out`` (fp32) and / or ``out_bf16``:
-    ``[rows, heads * head_dim]``. A row with no context gives zeros."""
+    ``[rows, heads * head_dim]``. A row with no context gives zeros. ``sinks`` (fp32 ``[heads]``): a logit
+    per head that takes weight and adds nothing (NaN makes the head NaN, +infinity zero)."""
     launches.add()
     kernels().kv4_attention(False, q, cache, block_tables, row_seq, row_ctx, scale, out, out_bf16, sinks, ws.status,
                             ws.part, ws.counters, ws.sms, PDL, ws.wait_polls)

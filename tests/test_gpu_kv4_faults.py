@@ -188,3 +188,25 @@ def test_outputs_whose_rows_lie_over_one_another_are_refused():
     a["q"] = a["q"][:1].expand(2, 8, 64)
     with pytest.raises(RuntimeError, match="over one another"):
         kv4.rope_append(*a.values())
+
+
+# ---- sinks that are not finite -------------------------------------------------------------------
+@pytest.mark.parametrize("fn", [kv4.attention_decode, kv4.attention_prefill])
+@pytest.mark.parametrize("spans", [[(40, 1)], [(9000, 1)], [(9000, 3), (0, 300), (77, 1)]])
+def test_sinks_that_are_not_finite(fn, spans):
+    """However a row's keys are divided up: a NaN sink gives NaN, one of +infinity takes all the weight, one of
+    -infinity none, and the other heads do not notice."""
+    case = _attention(64, spans)
+    ws, nan, inf = kv4.Workspace(DEV), float("nan"), float("inf")
+    sinks = torch.tensor([0.5, nan, inf, -inf, 3e38, -3e38, 2.0, -1.0], device=DEV)
+    out = []
+    for s in (sinks, torch.where(sinks.isfinite() & (sinks.abs() < 9), sinks, 0.0), None):
+        o = torch.zeros(case[0].shape[0], 8, 64, device=DEV)
+        fn(*case, 0.1, ws, out=o.view(-1, 512), sinks=s)
+        out.append(o)
+    got, finite, plain = out
+    assert got[:, 1].isnan().all() and not got[:, [0, 2, 3, 4, 5, 6, 7]].isnan().any()
+    assert (got[:, [2, 4]].abs() < 1e-30).all()
+    assert torch.equal(got[:, [0, 6, 7]], finite[:, [0, 6, 7]])
+    assert torch.allclose(got[:, [3, 5]], plain[:, [3, 5]], rtol=1e-6, atol=0)  # a sum of one term more
+    assert ws.status.item() == 0

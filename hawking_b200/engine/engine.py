@@ -384,9 +384,8 @@ class Engine:
         if k <= 0:
             self.spec = None
             return
-        if getattr(self.kv, "bits", 16) == 4:
-            # its attention cuts the batch's keys into equal ranges: a row's rounding depends on the batch
-            raise ValueError("speculative decoding needs the 16-bit KV cache (its output is bitwise the greedy output)")
+        from .speculative import check_cache
+        check_cache(self.kv)
         n = native()
         self.spec = {"k": max(1, min(k, n.MAX_VERIFY_BATCH - 1, m.max_rows - 1)),
                      "gov": n.SpecGovernor(16, min_accept_rate), "drafts": {}, "cycles": 0, "drafted": 0,
@@ -785,7 +784,7 @@ class Engine:
 
     def generate_speculative(self, prompt: List[int], params: Optional[SamplingParams] = None, k: int = 4):
         """Greedy generation of one prompt with n-gram speculative decoding (bitwise the greedy
-        output). Returns (tokens, SpecStats)."""
+        output; refused over the 4-bit KV cache). Returns (tokens, SpecStats)."""
         from .speculative import SpeculativeDecoder
         params = params or SamplingParams()
         dec = SpeculativeDecoder(self, k=k)

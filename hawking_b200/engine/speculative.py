@@ -41,8 +41,16 @@ class SpecStats:
         return self.emitted / self.cycles if self.cycles else 0.0
 
 
+def check_cache(kv) -> None:
+    """Refuse a cache over which the output would not be bitwise the greedy output: the 4-bit cache's
+    attention cuts a batch's keys into equal ranges, so a row's rounding depends on the rows beside it."""
+    if getattr(kv, "bits", 16) == 4:
+        raise ValueError("speculative decoding needs the 16-bit KV cache (its output is bitwise the greedy output)")
+
+
 class SpeculativeDecoder:
     def __init__(self, engine, k: int = 4, governor=None, min_accept_rate: float = 0.2):
+        check_cache(engine.kv)
         n = native()
         self.engine = engine
         self.k = max(0, min(k, n.MAX_VERIFY_BATCH - 1))

@@ -24,23 +24,25 @@ from typing import List, Optional
 
 def _cmd_generate(a) -> int:
     from ._ext import native
+    from .engine.kv_cache import KVBitsError
     from .engine.sampling import SamplingParams
     from .config import runtime_profile
     extra = {k: v for k, v in runtime_profile(a.profile).engine.items() if k != "max_batch"}
     if a.kv_bits != 16:
         extra["kv_bits"] = a.kv_bits
-    if a.gguf:
-        from .engine.engine import Engine
-        eng = Engine.from_gguf(a.gguf, max_batch=1, max_ctx=a.max_ctx, **extra)
-        tok = native().Tokenizer.from_gguf(native().GgufFile.open(a.gguf))
-    elif a.model:
-        from .serve.__main__ import path_engine
-        eng, tok = path_engine(a.model, 1, a.max_ctx, a.tokenizer_gguf, **extra)
-    else:
-        from .serve.__main__ import preset_engine
-        eng, tok = preset_engine(a.preset, a.layers, 1, a.max_ctx, **extra)
-    if getattr(eng.kv, "bits", 16) != a.kv_bits:
-        print(f"--kv-bits {a.kv_bits}: not available for this model's cache", file=sys.stderr)
+    try:
+        if a.gguf:
+            from .engine.engine import Engine
+            eng = Engine.from_gguf(a.gguf, max_batch=1, max_ctx=a.max_ctx, **extra)
+            tok = native().Tokenizer.from_gguf(native().GgufFile.open(a.gguf))
+        elif a.model:
+            from .serve.__main__ import path_engine
+            eng, tok = path_engine(a.model, 1, a.max_ctx, a.tokenizer_gguf, **extra)
+        else:
+            from .serve.__main__ import preset_engine
+            eng, tok = preset_engine(a.preset, a.layers, 1, a.max_ctx, **extra)
+    except KVBitsError as e:
+        print(f"--kv-bits {a.kv_bits}: not available for this model's cache ({e})", file=sys.stderr)
         return 2
     eng.apply_profile(a.profile)
     ids = tok.encode(a.prompt, True)

@@ -27,7 +27,7 @@ from .._ext import native
 from ..config import check_memory_budget, env_flag
 from ..models.config import ModelConfig
 from ..utils.trace import trace
-from .kv_cache import PagedKV4Cache, PagedKVCache
+from .kv_cache import PagedKV4Cache, PagedKVCache, check_kv_bits
 from .sampling import RequestRng, SamplingParams
 
 
@@ -112,8 +112,7 @@ class Engine:
             # MoE prefill decodes every expert once per forward (grouped tensor-core GEMMs):
             # prompts run in forwards of up to 2048 rows so that cost is shared by more tokens
             max_prefill_tokens = max(max_prefill_tokens, 2048)
-        if kv_bits not in (4, 16):
-            raise ValueError(f"kv_bits must be 16 or 4, not {kv_bits}")
+        check_kv_bits(kv_bits, cfg.arch)
         cache = PagedKV4Cache if kv_bits == 4 else PagedKVCache
         bpb = cache.bytes_per_block(cfg.layers, cfg.n_kv_heads, cfg.head_dim, block_size)
         free, _ = torch.cuda.mem_get_info(device)
@@ -192,6 +191,7 @@ class Engine:
             from ..models import qwen_next_artifact as qa
             if not qa.is_artifact(path):
                 raise ValueError(f"{path}: a .gravity artifact of an architecture this build does not load from files")
+            check_kv_bits(kw.get("kv_bits", 16), "qwen3next")
             cfg, w = qa.load(path, device, verify=verify)
             if max_ctx:
                 cfg = cfg.with_(max_ctx=max_ctx)
@@ -221,6 +221,7 @@ class Engine:
         ph["open"] = (time.perf_counter() - t) * 1e3
         t = time.perf_counter()
         cfg = config_from_gguf(m)
+        check_kv_bits(kw.get("kv_bits", 16), cfg.arch)
         if max_ctx:
             cfg = cfg.with_(max_ctx=max_ctx)
         ph["config"] = (time.perf_counter() - t) * 1e3

@@ -15,6 +15,18 @@ import torch
 from .._ext import native
 
 
+class KVBitsError(ValueError):
+    """A cache precision that a model cannot have."""
+
+
+def check_kv_bits(bits: int, arch: Optional[str] = None) -> None:
+    """Refuse a cache precision that does not exist, or that the models of ``arch`` have no cache in."""
+    if bits not in (4, 16):
+        raise KVBitsError(f"kv_bits must be 16 or 4, not {bits}")
+    if bits != 16 and arch in ("deepseek2", "qwen3next"):
+        raise KVBitsError(f"kv_bits={bits}: the models of architecture {arch} have a 16-bit cache only")
+
+
 class PagedKVCache:
     bits = 16
 

@@ -175,13 +175,15 @@ def preset_engine(preset: str, layers: int = 0, max_batch: int = 8, max_ctx=None
                   device="cuda", policy: int = 0, tp_rank: int = 0, tp_world: int = 1, **build_kw):
     """(Engine, tokenizer) for random-init weights of a named architecture preset. ``build_kw``
     (EngineConfig fields) reach the dense/MoE GGUF-architecture build; the MLA and hybrid engines
-    size their own prefill chunks. ``tp_world > 1``: this rank's tensor / expert parallel shard."""
+    size their own prefill chunks and have a 16-bit cache only. ``tp_world > 1``: this rank's tensor / expert parallel shard."""
     import os
     import tempfile
 
+    from ..engine.kv_cache import check_kv_bits
     from ..formats.synth import write_tokenizer_gguf
     from ..models.config import preset as get_preset
     cfg = get_preset(preset)
+    check_kv_bits(build_kw.get("kv_bits", 16), cfg.arch)
     if layers:
         cfg = cfg.with_(layers=layers)
     if max_ctx:

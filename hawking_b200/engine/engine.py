@@ -112,7 +112,7 @@ class Engine:
             # MoE prefill decodes every expert once per forward (grouped tensor-core GEMMs):
             # prompts run in forwards of up to 2048 rows so that cost is shared by more tokens
             max_prefill_tokens = max(max_prefill_tokens, 2048)
-        check_kv_bits(kv_bits, cfg.arch)
+        check_kv_bits(kv_bits, cfg.arch, cfg, block_size)
         cache = PagedKV4Cache if kv_bits == 4 else PagedKVCache
         bpb = cache.bytes_per_block(cfg.layers, cfg.n_kv_heads, cfg.head_dim, block_size)
         free, _ = torch.cuda.mem_get_info(device)
@@ -221,7 +221,7 @@ class Engine:
         ph["open"] = (time.perf_counter() - t) * 1e3
         t = time.perf_counter()
         cfg = config_from_gguf(m)
-        check_kv_bits(kw.get("kv_bits", 16), cfg.arch)
+        check_kv_bits(kw.get("kv_bits", 16), cfg.arch, cfg, kw.get("block_size", 64))
         if max_ctx:
             cfg = cfg.with_(max_ctx=max_ctx)
         ph["config"] = (time.perf_counter() - t) * 1e3

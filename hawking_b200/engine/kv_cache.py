@@ -8,6 +8,7 @@ the C++ ``BlockManager``; this class owns the memory and the device-side block t
 """
 from __future__ import annotations
 
+import math
 from typing import Dict, Iterable, List, Optional, Tuple
 
 import torch
@@ -19,12 +20,22 @@ class KVBitsError(ValueError):
     """A cache precision that a model cannot have."""
 
 
-def check_kv_bits(bits: int, arch: Optional[str] = None) -> None:
-    """Refuse a cache precision that does not exist, or that the models of ``arch`` have no cache in."""
+def check_kv_bits(bits: int, arch: str, cfg=None, block_size: int = 64) -> None:
+    """Refuse a cache precision that does not exist, that the models of ``arch`` have no cache in, or whose
+    kernels do not take the heads of ``cfg`` or the block size."""
     if bits not in (4, 16):
         raise KVBitsError(f"kv_bits must be 16 or 4, not {bits}")
     if bits != 16 and arch in ("deepseek2", "qwen3next"):
         raise KVBitsError(f"kv_bits={bits}: the models of architecture {arch} have a 16-bit cache only")
+    if bits == 4 and cfg is not None:
+        from ..ops import kv4
+        if cfg.n_heads % cfg.n_kv_heads or cfg.n_heads // cfg.n_kv_heads > kv4.MAX_GROUP:
+            raise KVBitsError(f"4-bit KV cache: a kv head serves at most {kv4.MAX_GROUP} query heads "
+                              f"({cfg.n_heads} query heads, {cfg.n_kv_heads} kv heads)")
+        try:
+            kv4.cache_shape(1, cfg.n_kv_heads, block_size, cfg.head_dim)
+        except ValueError as e:
+            raise KVBitsError(str(e)) from None
 
 
 class PagedKVCache:
@@ -113,7 +124,7 @@ class PagedKV4Cache(PagedKVCache):
     @staticmethod
     def bytes_per_block(layers: int, n_kv_heads: int, head_dim: int, block_size: int, elem_bytes: int = 2) -> int:
         from ..ops import kv4
-        return layers * n_kv_heads * (block_size // 16) * kv4.unit_bytes(head_dim)
+        return layers * math.prod(kv4.cache_shape(1, n_kv_heads, block_size, head_dim))
 
     def copy_blocks(self, pairs: List[Tuple[int, int]]):
         for src, dst in pairs:

@@ -183,7 +183,7 @@ def preset_engine(preset: str, layers: int = 0, max_batch: int = 8, max_ctx=None
     from ..formats.synth import write_tokenizer_gguf
     from ..models.config import preset as get_preset
     cfg = get_preset(preset)
-    check_kv_bits(build_kw.get("kv_bits", 16), cfg.arch)
+    check_kv_bits(build_kw.get("kv_bits", 16), cfg.arch, cfg, build_kw.get("block_size", 64))
     if layers:
         cfg = cfg.with_(layers=layers)
     if max_ctx:

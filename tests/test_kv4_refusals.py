@@ -80,3 +80,40 @@ def test_generate_refuses_before_it_loads(no_weights, tmp_path, capsys):
     for model in (["--gguf", gguf], ["--model", art], ["--preset", "deepseek-v3"], ["--preset", "qwen3-next"]):
         assert main(["generate", *model, "--prompt", "x", "--kv-bits", "4"]) == 2
         assert "not available for this model's cache" in capsys.readouterr().err
+
+
+# ---- heads and block sizes that the kernels do not take ------------------------------------------
+@pytest.mark.parametrize("heads,block_size,why", [(dict(n_heads=34, n_kv_heads=2), 64, "at most 16 query heads"),
+                                                  (dict(n_heads=20, n_kv_heads=8), 64, "at most 16 query heads"),
+                                                  (dict(head_dim=96), 64, "head_dim"), (dict(), 8, "multiple of 16"),
+                                                  (dict(), 24, "multiple of 16")])
+def test_engine_build_refuses_what_the_kernels_do_not_take(monkeypatch, heads, block_size, why):
+    """Before the pool is sized (8 tokens a block made its blocks 0 bytes) and before the first forward."""
+    import torch
+
+    from hawking_b200.models import llama
+    from hawking_b200.models.config import preset
+    from hawking_b200.serve.__main__ import preset_engine
+
+    def reached(*a, **k):
+        raise AssertionError("went on")
+
+    monkeypatch.setattr(torch.cuda, "mem_get_info", reached)
+    monkeypatch.setattr(llama, "random_llama_weights", reached)
+    cfg = preset("llama3-8b").with_(**heads)
+    with pytest.raises(ValueError, match=why):
+        Engine.build(cfg, None, device="cpu", block_size=block_size, kv_bits=4)
+    with pytest.raises(AssertionError):  # the 16-bit cache takes what it took
+        Engine.build(cfg, None, device="cpu", block_size=block_size)
+    if not heads:
+        with pytest.raises(ValueError, match=why):
+            preset_engine("llama3-8b", 1, kv_bits=4, block_size=block_size)
+        with pytest.raises(AssertionError):
+            preset_engine("llama3-8b", 1, block_size=block_size)
+
+
+def test_bytes_per_block_refuses_a_block_of_no_units():
+    from hawking_b200.engine.kv_cache import PagedKV4Cache
+    for bs in (0, 8, 24):
+        with pytest.raises(ValueError, match="multiple of 16"):
+            PagedKV4Cache.bytes_per_block(2, 2, 64, bs)

@@ -14,7 +14,8 @@ is written as its blocks' bytes (dtype "kv4", [layers, blocks, ...]) and restore
 the same size.
 
 ``PrefixDiskCache`` keeps such snapshots in a directory keyed by the rolling SHA-256 of the token
-prefix and finds the longest cached prefix of a new prompt (LRU by file time, bounded count).
+prefix and the kind of snapshot, and finds the longest cached prefix of a new prompt (LRU by file time,
+bounded count).
 
 ``save_recurrent`` / ``load_recurrent`` do the same for a hybrid model's fixed-size recurrent state
 (DeltaNet state and conv state of one sequence slot).
@@ -136,23 +137,31 @@ def load_sequence(kv, seq_id: int, path: str) -> List[int]:
     return tokens
 
 
-class PrefixDiskCache:
-    """Directory of KV snapshots keyed by the SHA-256 of each cached token prefix."""
+def snapshot_kind(kv) -> str:
+    """What a file name says of the caches that can load the snapshot: nothing of a 16-bit cache's, the block
+    size of a 4-bit cache's."""
+    return f".kv4-{kv.block_size}" if getattr(kv, "bits", 16) == 4 else ""
 
-    def __init__(self, directory: str, max_entries: int = 64):
+
+class PrefixDiskCache:
+    """Directory of KV snapshots keyed by the SHA-256 of each cached token prefix and by ``snapshot_kind``.
+    Lookups are for ``kv``'s kind (default: the 16-bit caches')."""
+
+    def __init__(self, directory: str, max_entries: int = 64, kv=None):
         self.dir = directory
         self.max_entries = max_entries
+        self.kind = snapshot_kind(kv)
         os.makedirs(directory, exist_ok=True)
 
     @staticmethod
     def key(tokens: Sequence[int]) -> str:
         return hashlib.sha256(np.asarray(tokens, dtype=np.int32).tobytes()).hexdigest()
 
-    def _path(self, tokens) -> str:
-        return os.path.join(self.dir, self.key(tokens) + ".hkkv")
+    def _path(self, tokens, kind: Optional[str] = None) -> str:
+        return os.path.join(self.dir, self.key(tokens) + (self.kind if kind is None else kind) + ".hkkv")
 
     def store(self, kv, seq_id: int, tokens: Sequence[int]) -> str:
-        p = self._path(tokens)
+        p = self._path(tokens, snapshot_kind(kv))
         save_sequence(kv, seq_id, tokens, p)
         self._evict()
         return p

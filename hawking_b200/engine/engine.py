@@ -285,12 +285,13 @@ class Engine:
         snapshot loaded into cache blocks and registered as a cached prefix, so the scheduler
         attaches it like any in-memory hit. When a prompt's prefill completes, its longest
         whole-block prefix of at least ``min_blocks`` blocks is written to disk (LRU over
-        ``max_entries`` files). Attention-only KV caches (no recurrent state).
+        ``max_entries`` files). Attention-only KV caches (no recurrent state). Engines of either cache
+        precision may share a directory: each finds its own snapshots.
 
         Parity: crates/hawking-core/src/cache/prefill_disk.rs:1-45 (rolling-hash prefix keys,
         longest-prefix lookup, LRU), crates/hawking-serve/src/http.rs:206-263 (lookup at admission)."""
         from .checkpoint import PrefixDiskCache
-        self.prefix_disk = PrefixDiskCache(directory, max_entries)
+        self.prefix_disk = PrefixDiskCache(directory, max_entries, self.kv)
         self._pd_min = max(1, min_blocks) * self.kv.block_size
         self._pd_pending: Dict[int, int] = {}  # request id -> prefix length to store after prefill
         self.stats_disk = {"hits": 0, "hit_tokens": 0, "stored": 0}

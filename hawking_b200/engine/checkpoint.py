@@ -10,8 +10,8 @@ corrupt or truncated file is refused, never half-loaded).
 File layout (little endian): b"HKKVSNP1" | u32 header_len | canonical JSON header | payload.
 The header holds the token ids, the cache geometry (layers, kv heads, head dim, dtype) and the
 payload digest; the payload is K then V, each [n_tokens, layers, kv_heads, head_dim] bf16. A cache in 4 bits
-is written as its blocks' bytes (dtype "kv4", [layers, blocks, ...]) and restored bit for bit into blocks of
-the same size.
+is written as its blocks' bytes (dtype "kv4", [layers, blocks, ...], zero past the last token) and restored bit
+for bit into blocks of the same size.
 
 ``PrefixDiskCache`` keeps such snapshots in a directory keyed by the rolling SHA-256 of the token
 prefix and the kind of snapshot, and finds the longest cached prefix of a new prompt (LRU by file time,
@@ -89,7 +89,13 @@ def save_sequence(kv, seq_id: int, tokens: Sequence[int], path: str) -> dict:
         raise ValueError("sequence holds fewer cached tokens than requested")
     if getattr(kv, "bits", 16) == 4:
         blocks = torch.tensor(kv.bm.table(seq_id)[: -(-n // kv.block_size)], dtype=torch.int64, device=kv.device)
-        payload = kv.data[:, blocks].contiguous().cpu().numpy().tobytes()
+        data = kv.data[:, blocks].contiguous().cpu()
+        tail = n % kv.block_size
+        if tail:  # the last block's other tokens are stale, another sequence's perhaps
+            from ..ops.kv4 import unit_tokens
+            of = 16 * torch.arange(kv.block_size // 16)[:, None] + unit_tokens(kv.hd)
+            data[:, -1, :, of >= tail] = 0
+        payload = data.numpy().tobytes()
         header = {"schema": "hawking_b200.kv_snapshot.v1", "tokens": [int(t) for t in tokens],
                   "layers": kv.layers, "kv_heads": kv.nkv, "head_dim": kv.hd, "dtype": "kv4",
                   "block_size": kv.block_size, "payload_bytes": len(payload),

@@ -44,6 +44,17 @@ def cache_shape(num_blocks: int, n_kv_heads: int, block_size: int, head_dim: int
     return num_blocks, n_kv_heads, block_size // 16, unit_bytes(head_dim)
 
 
+def unit_tokens(head_dim: int) -> torch.Tensor:
+    """The token (0 to 15) that each byte of a unit belongs to: no byte holds parts of two."""
+    unit_bytes(head_dim)
+    t, groups = torch.arange(16), head_dim // 64
+    keys = t.repeat_interleave(min(head_dim, 128) // 2).repeat(max(1, head_dim // 128))
+    # value words [group][g 8][t 4][i 2][h 2] hold tokens 8 h + 2 t (low half) and 8 h + 2 t + 1 (high half)
+    values = t.view(2, 4, 2).permute(1, 0, 2)[None, None, :, None, :, :, None].expand(groups, 8, 4, 2, 2, 2, 2)
+    pairs = t.repeat_interleave(4 * groups).repeat(2)
+    return torch.cat([keys, values.reshape(-1), pairs])
+
+
 class Workspace:
     """What the attention launches of one stream share: the device status word, the partial results of
     rows that several CTAs work on, and their arrival counters (zero between launches). Use one

@@ -76,10 +76,12 @@ struct Kv4Workspace {
   int sms;
 };
 constexpr int kKv4Counters = 2048;  // decode: three per CTA
-// decode: one CTA per SM, with two partials of its own and one of each of its 15 warps (11 where a partial is
-// larger), of at most 16 heads x (128 + 4) or 8 x (256 + 4) floats
-// prefill with split keys: at most one part of 256 rows x (128 + 4) per SM
-constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * 256 * 132; }
+// Floats per SM. Decode: one CTA, with two partials of its own and one of each of its 15 warps (11 at head_dim 256), of
+// an item's heads (at most kKv4ItemHeads: more per kv head make two items) x (head_dim + 4). Prefill with split keys: at
+// most one part of 256 rows x (128 + 4).
+constexpr int kKv4ItemHeads = 8;
+constexpr int kKv4PartFloatsPerSm = 256 * 132;
+constexpr int64_t kKv4PartFloats(int sms) { return (int64_t)sms * kKv4PartFloatsPerSm; }
 
 void kv4_plan_launch(const Kv4PlanArgs& a, cudaStream_t s, bool pdl);
 void kv4_append_launch(const Kv4AppendArgs& a, cudaStream_t s, bool pdl);

@@ -118,7 +118,8 @@ struct DecodeShape {
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kSmem = kWarps * kRing;  // the ring's place takes the part's last partial
   static_assert(kSmem + 10 * 1024 <= 227 * 1024, "shared memory of an SM");
-  static_assert(8 * kRow * 4 <= kRing, "the last partial fits the ring");
+  static_assert(kKv4ItemHeads * kRow * 4 <= kRing, "the last partial fits the ring");
+  static_assert((2 + kWarps) * kKv4ItemHeads * kRow <= kKv4PartFloatsPerSm, "a CTA's partials fit the workspace");
 };
 
 // A warp's partial in shared memory: units [u0, u1) of a pair.
@@ -865,8 +866,8 @@ void kv4_attention_decode_launch(const Kv4AttnArgs& args, const Kv4Workspace& ws
     if (d.a.out_bf16) d.a.out_bf16 += r0 * args.out_stride;
     d.part = ws.part;
     d.counters = ws.counters;
-    d.heads_per_item = G < 8 ? G : 8;
-    d.split = G > 8 ? 1 : 0;
+    d.heads_per_item = G < kKv4ItemHeads ? G : kKv4ItemHeads;
+    d.split = G > kKv4ItemHeads ? 1 : 0;
     const int upb = args.block_size / 16;
     d.upb_shift = (upb & (upb - 1)) ? -1 : __builtin_ctz(upb);
     if (args.hd == 64) launch_decode<64>(d, ws.sms, s, pdl);

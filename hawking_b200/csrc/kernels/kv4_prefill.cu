@@ -76,6 +76,7 @@ struct PrefillShape {
   static constexpr int kOffK = 2 * kQTile;
   static constexpr int kOffV = kOffK + 2 * kKStage;
   static constexpr int kSmem = kOffV + 2 * kVStage + 1024;  // + alignment
+  static_assert(kRows * (HD + 4) <= kKv4PartFloatsPerSm, "a CTA's part fits the workspace");
 };
 
 __device__ __forceinline__ float ex2(float x) {

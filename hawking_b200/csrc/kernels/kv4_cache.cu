@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(Kv4PlanArgs a) {
 // A warp takes HB heads of one row (HB pairs of heads at HD 64), so that the position's rotation is read once
 // for them and all their loads are in flight together: at 2048 rows of 48 heads of 128 in the L2 cache HB = 4 took
 // 17 us, 2 took 21, 1 took 31. A few rows keep one head per warp (the launch needs warps more than the warps work).
-// 2048 rows of 32 / 8 heads of 128 took 20 us (70 MB: 11), bound by instructions: issue slots 63 % busy, the ALU 45 %.
+// 2048 rows of 32 / 8 heads of 128 took 20 us (70 MB: 11): issue slots 63 % busy, the ALU 45 %, and 30 % of a warp's time
+// waiting for loads that nothing overlaps, at the half occupancy of 60 registers.
 // An instance per rotation style, with and without bias and norms: deciding both in the kernel took 25 us instead of 17
 // in the L2 cache. Codes come from a reciprocal, with the exact division only near half-way between two codes.
 // Every lane holds 4 consecutive dims of each 128 (or 64), 16 lanes the 64 dims of a quantisation group.

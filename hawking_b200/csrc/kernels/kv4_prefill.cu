@@ -26,7 +26,7 @@
 // softmax threads need 168 registers, which the unpackers (112) and the issuing warpgroup (64) give up. Four unpacking
 // warps keep ahead of the products; with eight, in 640 threads, the softmax threads spilled and it was slower.
 //
-// What bounds it, on one B200, 32 / 8 heads of 128. 2048 rows after 6144 tokens: 301 us, 0.8 PFLOP/s, 0.49 of the
+// What bounds it, on one B200, 32 / 8 heads of 128. 2048 rows after 6144 tokens: 299 us, 0.8 PFLOP/s, 0.49 of the
 // measured bf16 rate. 256 equal CTAs on 148 SMs take two turns where 1.73 would do; within a CTA 128 keys take 2.8 us,
 // the exchange of scores and weights through tensor memory 48 % busy and issue slots 47 %: the softmax of a tile, not
 // the products (1.8 us by themselves), paces the loop. A CTA's begin (queries fetched and scaled, first keys unpacked) takes 6 us and its

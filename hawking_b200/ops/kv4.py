@@ -9,9 +9,10 @@ of its block tables, from the request lengths), then per layer ``rope_append`` a
 ``attention_decode`` (rows that are one token of a sequence each) or ``attention_prefill`` (runs of
 rows of one sequence). ``gather`` reads tokens back as bf16 rows.
 
-Every function launches on the current CUDA stream. Kernels report bad device-side indices through
-a status word (``Workspace.status``, or the ``status`` argument of ``plan_rows``) and never follow
-them.
+Every function launches on the current CUDA stream. Kernels never follow bad device-side indices.
+``plan_rows`` and the attention report them in a status word (the ``status`` argument,
+``Workspace.status``: 4); ``rope_append`` skips such rows and ``gather`` gives zeros, without a word. A
+context past the end of its table row is taken as the table row's length.
 
 Parity: crates/hawking-core/shaders/mha.metal (int4 KV decode, per-row scales),
 workspace/docs/reference/env_flags.md:29-35 (the int4 KV mode).
